@@ -44,7 +44,7 @@ def _compile(src: Path, verbose: bool) -> Path:
     obj = BUILD / (src.name + ".o")
     cmd = [HIPCC, *COMMON]
     if src.suffix == ".cpp":
-        cmd += ["-x", "hip"] if src.name == "api.cpp" else []
+        cmd += ["-x", "hip"] if src.name in ("api.cpp", "api_decode.cpp") else []
     cmd += ["-c", str(src), "-o", str(obj)]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -391,6 +391,10 @@ const char *device_error_text(uint32_t code) {
     case sihip::kDevErrCombineWait: return "a kernel gave up waiting for a split tile's partial sums";
     case sihip::kDevErrArgmaxWait: return "a kernel gave up waiting for a workgroup's argmax candidate";
     case sihip::kDevErrTokenId: return "an embedding token id lies beyond the table";
+    case sihip::kDevErrCachePage: return "a page table entry lies beyond the cache's pool";
+    case sihip::kDevErrCacheFull: return "a sequence's tokens do not fit its pages";
+    case sihip::kDevErrDraftToken: return "a drafted token id lies beyond the vocabulary";
+    case sihip::kDevErrNoMass: return "a row of probabilities is zero throughout";
     default: return "a kernel reported an unknown failure";
   }
 }
@@ -498,6 +502,20 @@ int dispatch_gate_up(si_hip_context *ctx, const uint8_t *g, const uint8_t *u, co
 hipStream_t device_stream(const si_hip_context *ctx) {
   return ctx->capturing ? ctx->capture_stream : ctx->stream;
 }
+}  // namespace
+
+namespace sihip {
+int submit_device(si_hip_context *ctx, const char *what, DeviceLaunch launch, void *arg) {
+  if (!ctx) return fail(SI_HIP_ERR_NULL, "HIP context is null");
+  CallScope scope(ctx);
+  const hipError_t e = launch(arg, ctx->ws, device_stream(ctx), ctx->policy == SI_HIP_KERNEL_AUTO);
+  if (e != hipSuccess) return hip_fail(e, what);
+  ctx->async_submitted.fetch_add(1);
+  return ok();
+}
+}  // namespace sihip
+
+namespace {
 
 // Validation shared by the byte-slice matvec entry points
 // (quant_k_matvec_dispatch, metal.rs:3847-3858 and 3884-3887).

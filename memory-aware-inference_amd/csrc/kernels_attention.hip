@@ -1,0 +1,193 @@
+// Attention of a sequence's new tokens over its paged cache.
+//
+// out = sum_i p_i v_i, p_i = exp(scale q.k_i - m) / l, over the slots a row
+// sees; m and l run along with the slots, and every sum is held in 32 bits.
+// Scores are taken times log2(e), so that p is an exp2.
+//
+// Rows of one kv head: row r = t * group + g is token t's query head
+// kv_head * group + g.
+#include "decode_internal.h"
+
+namespace sihip {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kThreads = 256;
+
+// ---- workspace --------------------------------------------------------------
+// With weights: (m, 1 / l) of every row, then its scores of all slots, both
+// [sequences][kv_heads][rows].
+struct Space {
+  size_t stats, scores, bytes;
+  uint32_t score_stride;
+};
+Space space_of(const CacheView& c, uint32_t heads, uint32_t tokens, bool weights) {
+  Space s{};
+  const size_t rows = (size_t)c.sequences * heads * tokens;
+  s.score_stride = (c.capacity + 3u) / 4u * 4u;
+  if (weights) {
+    s.stats = s.bytes;
+    s.bytes += (rows * 8u + 255u) / 256u * 256u;
+    s.scores = s.bytes;
+    s.bytes += rows * s.score_stride * 4u;
+  }
+  return s;
+}
+
+// The slots that token t of a sequence of `length` tokens sees: [begin, end).
+__device__ __forceinline__ void seen_slots(uint32_t length, uint32_t t, uint32_t capacity,
+                                           uint32_t window, uint32_t& begin, uint32_t& end) {
+  const uint32_t n = length + t + 1u;
+  end = min(n, capacity);
+  begin = window != 0u && n > window ? n - window : 0u;
+}
+
+template <typename T>
+__device__ __forceinline__ float value_of(T v);
+template <>
+__device__ __forceinline__ float value_of<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float value_of<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float value_of<__hip_bfloat16>(__hip_bfloat16 v) {
+  return __bfloat162float(v);
+}
+
+template <bool MAX>
+__device__ __forceinline__ float block_reduce(float v, float* part) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float w = __shfl_xor(v, o, 64);
+    v = MAX ? fmaxf(v, w) : v + w;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63u) == 0u) part[threadIdx.x / 64u] = v;
+  __syncthreads();
+  float r = part[0];
+#pragma unroll
+  for (uint32_t i = 1; i < kThreads / 64u; ++i) r = MAX ? fmaxf(r, part[i]) : r + part[i];
+  return r;
+}
+
+// ---- one workgroup a row, any head size and alignment --------------------------
+// grid (heads, tokens, sequences).  A thread takes a slot's score, then a
+// value of the head's output.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_generic(AttentionArgs a, float2* stats,
+                                                              float* scores,
+                                                              uint32_t score_stride) {
+  __shared__ float q[kMaxHeadDim], p[kThreads], part[kThreads / 64];
+  __shared__ uint32_t row[kThreads];
+  const CacheView& c = a.cache;
+  const uint32_t h = blockIdx.x, t = blockIdx.y, s = blockIdx.z, dim = c.head_dim;
+  const uint32_t kv = h / a.group, i = threadIdx.x;
+  float* out = a.out + (((size_t)s * a.tokens + t) * a.heads + h) * dim;
+  const uint32_t rows = a.tokens * a.group, r = t * a.group + (h - kv * a.group);
+  const size_t at = ((size_t)s * c.kv_heads + kv) * rows + r;
+  float* score = scores ? scores + at * score_stride : nullptr;
+  const uint32_t count = brought(a.counts, s, a.tokens);
+  if (t >= count) {
+    if (i < dim) out[i] = 0.0f;
+    if (stats && i == 0u) stats[at] = make_float2(0.0f, 0.0f);
+    return;
+  }
+  if (t == 0u && h == 0u && i == 0u &&
+      (uint64_t)c.lengths[s] + count > c.capacity)
+    report_device_error(a.report, kDevErrCacheFull);
+  uint32_t begin, end;
+  seen_slots(held(c, s), t, c.capacity, a.window, begin, end);
+  const float scale = a.scale * kLog2e;
+  if (i < dim)
+    q[i] = a.q[((size_t)s * a.tokens + t) * a.q_token_stride + h * a.q_head_stride + i] * scale;
+  float m = -INFINITY, l = 0.0f, acc = 0.0f;
+  bool any = false, bad = false;
+  for (uint32_t base = begin; base < end; base += kThreads) {
+    const uint32_t slot = base + i;
+    uint32_t at_row = kNone;
+    if (slot < end) {
+      at_row = cache_row(c, s, kv, slot);
+      bad |= at_row == kNone;
+    }
+    __syncthreads();  // the values of the last tile are taken, and q is there
+    row[i] = at_row;
+    float v = -INFINITY;
+    if (at_row != kNone) {
+      const T* key = static_cast<const T*>(c.keys) + (size_t)at_row * dim;
+      v = 0.0f;
+      for (uint32_t d = 0; d < dim; ++d) v = fmaf(q[d], value_of<T>(key[d]), v);
+    }
+    if (score && slot < end) score[slot] = v;
+    any |= __syncthreads_or(at_row != kNone) != 0;
+    const float top = fmaxf(m, block_reduce<true>(v, part));
+    const float from = top == -INFINITY ? 0.0f : top;
+    const float e = at_row != kNone ? exp2f(v - from) : 0.0f;
+    const float keep = exp2f(m - from);
+    p[i] = e;
+    l = l * keep + block_reduce<false>(e, part);  // (its barriers publish p and row)
+    m = top;
+    acc *= keep;
+    if (i < dim)
+      for (uint32_t j = 0; j < min(kThreads, end - base); ++j)
+        if (row[j] != kNone)
+          acc = fmaf(p[j], value_of<T>(static_cast<const T*>(c.values)[(size_t)row[j] * dim + i]),
+                     acc);
+  }
+  if (bad) report_device_error(a.report, kDevErrCachePage);
+  if (i < dim) out[i] = any ? acc / l : 0.0f;
+  if (stats && i == 0u)
+    stats[at] = any ? make_float2(m == -INFINITY ? 0.0f : m, 1.0f / l) : make_float2(0.0f, 0.0f);
+}
+
+// weights[slot] += sum over the kv head's rows of exp2(score - m) / l, rows in
+// their order.  grid (slots / 256, kv_heads, sequences).
+__global__ __launch_bounds__(kThreads) void attention_weights(AttentionArgs a, const float2* stats,
+                                                              const float* scores,
+                                                              uint32_t score_stride) {
+  const CacheView& c = a.cache;
+  const uint32_t slot = blockIdx.x * kThreads + threadIdx.x, kv = blockIdx.y, s = blockIdx.z;
+  const uint32_t count = brought(a.counts, s, a.tokens), length = held(c, s);
+  const uint32_t rows = a.tokens * a.group;
+  if (count == 0u || slot >= min(length + count, c.capacity)) return;
+  const size_t at = ((size_t)s * c.kv_heads + kv) * rows;
+  float sum = 0.0f;
+  for (uint32_t t = 0; t < count; ++t) {
+    uint32_t begin, end;
+    seen_slots(length, t, c.capacity, a.window, begin, end);
+    if (slot < begin || slot >= end) continue;
+    for (uint32_t g = 0; g < a.group; ++g) {
+      const size_t r = at + t * a.group + g;
+      const float2 st = stats[r];
+      if (st.y != 0.0f) sum += exp2f(scores[r * score_stride + slot] - st.x) * st.y;
+    }
+  }
+  a.weights[((size_t)s * c.kv_heads + kv) * a.weights_stride + slot] += sum;
+}
+
+}  // namespace
+
+size_t attention_workspace_bytes(const CacheView& cache, uint32_t heads, uint32_t tokens,
+                                 bool weights) {
+  return std::max(space_of(cache, heads, tokens, weights).bytes, size_t(16));
+}
+
+hipError_t launch_attention(const AttentionArgs& a, bool tuned, hipStream_t s) {
+  const CacheView& c = a.cache;
+  const Space sp = space_of(c, a.heads, a.tokens, a.weights != nullptr);
+  uint8_t* w = static_cast<uint8_t*>(a.workspace);
+  float2* stats = a.weights ? reinterpret_cast<float2*>(w + sp.stats) : nullptr;
+  float* scores = a.weights ? reinterpret_cast<float*>(w + sp.scores) : nullptr;
+  const dim3 grid(a.heads, a.tokens, c.sequences);
+  if (c.type == kKvF32)
+    attention_generic<float><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
+  else if (c.type == kKvF16)
+    attention_generic<__half><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
+  else
+    attention_generic<__hip_bfloat16><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.weights) return e;
+  attention_weights<<<dim3((c.capacity + kThreads - 1u) / kThreads, c.kv_heads, c.sequences),
+                      kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
+  return hipGetLastError();
+}
+
+}  // namespace sihip

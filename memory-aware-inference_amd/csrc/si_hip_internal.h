@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+struct si_hip_context;  // api.cpp
+
 namespace sihip {
 
 // Device memory a context lends to the kernels that combine partial sums
@@ -52,6 +54,10 @@ enum DeviceError : uint32_t {
   kDevErrCombineWait = 2,  // a split tile's partial sums did not arrive
   kDevErrArgmaxWait = 3,   // a workgroup's argmax candidate did not arrive
   kDevErrTokenId = 4,      // an embedding token id beyond the table
+  kDevErrCachePage = 5,    // a page table entry beyond a cache's pool
+  kDevErrCacheFull = 6,    // a sequence's tokens do not fit its pages
+  kDevErrDraftToken = 7,   // a drafted token id beyond the vocabulary
+  kDevErrNoMass = 8,       // a row of probabilities that is zero throughout
 };
 
 // Stores `code` into the workspace owner's error word (a system-scope store
@@ -112,6 +118,13 @@ __host__ __device__ __forceinline__ uint32_t argmax_candidate_index(uint64_t c, 
 // noalloc.hip: sets up the current device's workspace of
 // si_hip_quant_matvec_noalloc (once per device; `stream` not under capture).
 int noalloc_setup(hipStream_t stream);
+
+// api.cpp: runs `launch(arg, workspace, stream, tuned)` as one device call of the
+// context: under its lock, on its compute stream or, while a capture is open,
+// its capture stream; `tuned` is false under the generic kernel policy.
+// Returns the call's status.
+using DeviceLaunch = hipError_t (*)(void* arg, const Workspace& ws, hipStream_t stream, bool tuned);
+int submit_device(si_hip_context* ctx, const char* what, DeviceLaunch launch, void* arg);
 
 // kernels_generic.hip
 hipError_t launch_matvec_generic(uint32_t type, const uint8_t* w, const float* x, float* y,

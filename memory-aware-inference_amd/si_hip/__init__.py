@@ -22,6 +22,9 @@ _HERE = Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libsi_hip.so"
 INCLUDE_DIR = _HERE.parent.parent / "include"
 
+GGML_TYPE_F32 = 0
+GGML_TYPE_F16 = 1
+GGML_TYPE_BF16 = 30
 GGML_TYPE_Q4_K = 12
 GGML_TYPE_Q5_K = 13
 GGML_TYPE_Q6_K = 14
@@ -32,6 +35,14 @@ KERNEL_AUTO = 0
 KERNEL_GENERIC = 1
 DEFAULT_RESIDENCY_BUDGET = 16 << 30  # SI_HIP_DEFAULT_RESIDENCY_BUDGET
 MAX_BATCH = 16
+MAX_HEAD_DIM = 256
+MAX_STEP_TOKENS = 16
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
+ROPE_SCALING_NONE = 0
+ROPE_SCALING_LINEAR = 1
+ROPE_SCALING_YARN = 2
+TOKEN_NONE = 0xFFFFFFFF
 
 STATUS = {
     0: "SI_HIP_OK", -1: "SI_HIP_ERR_NULL", -2: "SI_HIP_ERR_DIMENSIONS",
@@ -58,6 +69,29 @@ class ResidencyStats(C.Structure):
     _fields_ = [("hits", C.c_uint64), ("uploads", C.c_uint64), ("uploaded_bytes", C.c_uint64),
                 ("evictions", C.c_uint64), ("resident_ranges", C.c_uint64),
                 ("resident_bytes", C.c_uint64), ("budget_bytes", C.c_uint64)]
+
+
+class KvCache(C.Structure):
+    """A paged key-value cache in device memory that the caller owns
+    (si_hip_kv_cache): device addresses and the pool's shape."""
+
+    _fields_ = [("ggml_type", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_tokens", C.c_uint32), ("pages", C.c_uint32), ("sequences", C.c_uint32),
+                ("max_pages", C.c_uint32), ("reserved", C.c_uint32), ("d_keys", C.c_void_p),
+                ("d_values", C.c_void_p), ("d_page_table", C.c_void_p),
+                ("d_lengths", C.c_void_p)]
+
+    @property
+    def capacity(self) -> int:
+        """Slots a sequence has."""
+        return self.max_pages * self.page_tokens
+
+
+class Rope(C.Structure):
+    """A rotation by positions (si_hip_rope); rope_frequencies makes its table."""
+
+    _fields_ = [("layout", C.c_uint32), ("rotary_dim", C.c_uint32), ("magnitude", C.c_float),
+                ("reserved", C.c_uint32), ("d_frequencies", C.c_void_p)]
 
 
 class GgufValueC(C.Structure):
@@ -171,6 +205,21 @@ _SIGS = {
     "si_hip_gguf_quant_matvec_many_bytes": (
         _I, [_P, C.POINTER(C.c_uint32), C.POINTER(_BP), C.POINTER(_SZ), C.POINTER(_SZ),
              C.POINTER(_SZ), _SZ, _FP, _SZ, C.POINTER(_FP)]),
+    # si_hip_decode.h
+    "si_hip_rope_frequencies": (_I, [_SZ, C.c_double, _U32, C.c_double, C.c_double, C.c_double,
+                                     C.c_double, C.POINTER(_U64), _FP]),
+    "si_hip_rope_device": (_I, [_P, C.POINTER(Rope), _P, _SZ, _SZ, _SZ, _SZ, _SZ, _P, _P, _SZ,
+                                _SZ]),
+    "si_hip_rope_append_device": (_I, [_P, C.POINTER(KvCache), C.POINTER(Rope), _SZ, _P, _P, _P,
+                                       _SZ, _P, _SZ, _P, _SZ, _SZ, _SZ, _P]),
+    "si_hip_kv_advance_device": (_I, [_P, C.POINTER(KvCache), _P, _U32]),
+    "si_hip_paged_attention_workspace": (_SZ, [C.POINTER(KvCache), _SZ, _SZ, _I]),
+    "si_hip_paged_attention_device": (_I, [_P, C.POINTER(KvCache), _SZ, _SZ, _U32, C.c_float, _P,
+                                           _P, _SZ, _SZ, _P, _P, _SZ, _P, _SZ]),
+    "si_hip_kv_evict_device": (_I, [_P, C.POINTER(KvCache), _P, _SZ, _SZ, _SZ, _SZ,
+                                    C.POINTER(KvCache), _P, _SZ, _P]),
+    "si_hip_softmax_device": (_I, [_P, _P, _SZ, _SZ, C.c_float, _P]),
+    "si_hip_verify_draft_device": (_I, [_P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _P, _P]),
     # si_hip_gguf.h
     "si_hip_gguf_open": (_I, [C.c_char_p, C.POINTER(_P)]),
     "si_hip_gguf_parse": (_I, [_BP, _SZ, C.POINTER(_P)]),
@@ -290,6 +339,20 @@ def f32_to_f16_bits(v: float) -> int:
 
 
 # ---------------------------------------------------------------------------
+
+def rope_frequencies(rotary_dim: int, theta: float, scaling: int = ROPE_SCALING_NONE,
+                     factor: float = 1.0, original_length: float = 0.0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """A rotation's frequency table (host uint64, to be copied to the device)
+    and the magnitude that goes with it."""
+    table = np.empty(max(rotary_dim // 2, 1), dtype=np.uint64)
+    magnitude = C.c_float()
+    _check(lib().si_hip_rope_frequencies(rotary_dim, theta, scaling, factor, original_length,
+                                         beta_fast, beta_slow,
+                                         table.ctypes.data_as(C.POINTER(_U64)),
+                                         C.byref(magnitude)))
+    return table, float(magnitude.value)
+
 
 class QuantWeight:
     """Owning handle of HBM-resident packed blocks (QuantWeight, metal.rs:1840)."""
@@ -640,6 +703,85 @@ class HipContext:
         y = np.empty(max(elements, 1), dtype=np.float32)
         _check(lib().si_hip_dequantize(self._h, ggml_type, _bp(b), b.size, elements, _fp(y)))
         return y[:elements]
+
+    # ---- the operators around a decode step's projections (include/si_hip_decode.h)
+    def rope_device(self, rope: Rope, d_x: int, tokens: int, heads: int, head_dim: int,
+                    d_positions: int, d_y: int, token_stride: int | None = None,
+                    head_stride: int | None = None, y_token_stride: int | None = None,
+                    y_head_stride: int | None = None) -> None:
+        """Rotates rows of heads by their positions; strides are in floats and
+        default to contiguous rows."""
+        hs = head_dim if head_stride is None else head_stride
+        yhs = head_dim if y_head_stride is None else y_head_stride
+        _check(lib().si_hip_rope_device(
+            self._h, rope, d_x, tokens, heads, head_dim,
+            heads * hs if token_stride is None else token_stride, hs, d_positions, d_y,
+            heads * yhs if y_token_stride is None else y_token_stride, yhs))
+
+    def rope_append_device(self, cache: KvCache, tokens: int, d_k: int, d_v: int,
+                           rope: Rope | None = None, d_counts: int | None = None,
+                           d_positions: int | None = None, k_token_stride: int | None = None,
+                           v_token_stride: int | None = None, d_q: int | None = None,
+                           heads: int = 0, q_token_stride: int | None = None,
+                           q_head_stride: int | None = None, d_q_out: int | None = None) -> None:
+        """New tokens' keys (rotated) and values into the cache behind its
+        lengths, and their query rows rotated into d_q_out."""
+        row = cache.kv_heads * cache.head_dim
+        qhs = cache.head_dim if q_head_stride is None else q_head_stride
+        _check(lib().si_hip_rope_append_device(
+            self._h, cache, rope, tokens, d_counts, d_positions, d_k,
+            row if k_token_stride is None else k_token_stride, d_v,
+            row if v_token_stride is None else v_token_stride, d_q, heads,
+            heads * qhs if q_token_stride is None else q_token_stride, qhs, d_q_out))
+
+    def kv_advance_device(self, cache: KvCache, d_counts: int | None = None,
+                          more: int = 0) -> None:
+        """Lengths grow by d_counts and `more`."""
+        _check(lib().si_hip_kv_advance_device(self._h, cache, d_counts, more))
+
+    def paged_attention_workspace(self, cache: KvCache, heads: int, tokens: int,
+                                  with_weights: bool = False) -> int:
+        """Bytes of device scratch that paged_attention_device needs."""
+        n = lib().si_hip_paged_attention_workspace(cache, heads, tokens, int(with_weights))
+        if n == 0:
+            raise HipError(-2, last_error())
+        return int(n)
+
+    def paged_attention_device(self, cache: KvCache, heads: int, tokens: int, scale: float,
+                               d_q: int, d_out: int, d_workspace: int, workspace_bytes: int,
+                               window: int = 0, d_counts: int | None = None,
+                               q_token_stride: int | None = None,
+                               q_head_stride: int | None = None, d_weights: int | None = None,
+                               weights_stride: int = 0) -> None:
+        """Attention of each sequence's new tokens over its cache; with
+        d_weights the cached tokens' weights are added up there."""
+        qhs = cache.head_dim if q_head_stride is None else q_head_stride
+        _check(lib().si_hip_paged_attention_device(
+            self._h, cache, heads, tokens, window, scale, d_counts, d_q,
+            heads * qhs if q_token_stride is None else q_token_stride, qhs, d_out, d_weights,
+            weights_stride, d_workspace, workspace_bytes))
+
+    def kv_evict_device(self, cache: KvCache, d_weights: int, weights_stride: int, keep: int,
+                        sinks: int, recent: int, to: KvCache, d_to_weights: int,
+                        to_weights_stride: int, d_kept: int) -> None:
+        """The tokens of each head that weigh most, moved to the cache `to`."""
+        _check(lib().si_hip_kv_evict_device(self._h, cache, d_weights, weights_stride, keep,
+                                            sinks, recent, to, d_to_weights, to_weights_stride,
+                                            d_kept))
+
+    def softmax_device(self, d_x: int, rows: int, cols: int, temperature: float,
+                       d_y: int) -> None:
+        _check(lib().si_hip_softmax_device(self._h, d_x, rows, cols, temperature, d_y))
+
+    def verify_draft_device(self, d_target: int, d_draft: int | None, d_tokens: int,
+                            d_uniform: int, sequences: int, drafts: int, vocab: int,
+                            d_accepted: int, d_out_tokens: int,
+                            d_counts: int | None = None) -> None:
+        """Drafted tokens against the target's probabilities: how many are
+        accepted, and the tokens that follow."""
+        _check(lib().si_hip_verify_draft_device(self._h, d_target, d_draft, d_tokens, d_counts,
+                                                d_uniform, sequences, drafts, vocab, d_accepted,
+                                                d_out_tokens))
 
     # ---- device-resident plumbing
     def device_alloc(self, nbytes: int) -> int:
