@@ -6,41 +6,14 @@
 //
 // Rows of one kv head: row r = t * group + g is token t's query head
 // kv_head * group + g.
-#include "decode_internal.h"
+#include "attention_common.h"
 
 namespace sihip {
+using namespace attn;
+
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kThreads = 256;
-
-// ---- workspace --------------------------------------------------------------
-// With weights: (m, 1 / l) of every row, then its scores of all slots, both
-// [sequences][kv_heads][rows].
-struct Space {
-  size_t stats, scores, bytes;
-  uint32_t score_stride;
-};
-Space space_of(const CacheView& c, uint32_t heads, uint32_t tokens, bool weights) {
-  Space s{};
-  const size_t rows = (size_t)c.sequences * heads * tokens;
-  s.score_stride = (c.capacity + 3u) / 4u * 4u;
-  if (weights) {
-    s.stats = s.bytes;
-    s.bytes += (rows * 8u + 255u) / 256u * 256u;
-    s.scores = s.bytes;
-    s.bytes += rows * s.score_stride * 4u;
-  }
-  return s;
-}
-
-// The slots that token t of a sequence of `length` tokens sees: [begin, end).
-__device__ __forceinline__ void seen_slots(uint32_t length, uint32_t t, uint32_t capacity,
-                                           uint32_t window, uint32_t& begin, uint32_t& end) {
-  const uint32_t n = length + t + 1u;
-  end = min(n, capacity);
-  begin = window != 0u && n > window ? n - window : 0u;
-}
 
 template <typename T>
 __device__ __forceinline__ float value_of(T v);
@@ -167,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void attention_weights(AttentionArgs a, c
 
 size_t attention_workspace_bytes(const CacheView& cache, uint32_t heads, uint32_t tokens,
                                  bool weights) {
-  return std::max(space_of(cache, heads, tokens, weights).bytes, size_t(16));
+  return space_of(cache, heads, tokens, weights).bytes;
 }
 
 hipError_t launch_attention(const AttentionArgs& a, bool tuned, hipStream_t s) {
@@ -176,14 +149,21 @@ hipError_t launch_attention(const AttentionArgs& a, bool tuned, hipStream_t s) {
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   float2* stats = a.weights ? reinterpret_cast<float2*>(w + sp.stats) : nullptr;
   float* scores = a.weights ? reinterpret_cast<float*>(w + sp.scores) : nullptr;
-  const dim3 grid(a.heads, a.tokens, c.sequences);
-  if (c.type == kKvF32)
-    attention_generic<float><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
-  else if (c.type == kKvF16)
-    attention_generic<__half><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
-  else
-    attention_generic<__hip_bfloat16><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
-  hipError_t e = hipGetLastError();
+  bool taken = false;
+  hipError_t e = hipSuccess;
+  if (tuned) e = launch_attention_mfma(a, sp, &taken, s);
+  if (e != hipSuccess) return e;
+  if (!taken) {
+    const dim3 grid(a.heads, a.tokens, c.sequences);
+    if (c.type == kKvF32)
+      attention_generic<float><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
+    else if (c.type == kKvF16)
+      attention_generic<__half><<<grid, kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
+    else
+      attention_generic<__hip_bfloat16><<<grid, kThreads, 0, s>>>(a, stats, scores,
+                                                                  sp.score_stride);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess || !a.weights) return e;
   attention_weights<<<dim3((c.capacity + kThreads - 1u) / kThreads, c.kv_heads, c.sequences),
                       kThreads, 0, s>>>(a, stats, scores, sp.score_stride);
