@@ -1,0 +1,10 @@
+// Attention over a paged F16 cache (attention_mfma.h).
+#include "attention_mfma.h"
+
+namespace sihip {
+
+hipError_t launch_attention_f16(const AttentionArgs& a, const attn::Outputs& o, hipStream_t s) {
+  return attn::launch_type<attn::F16>(a, o, s);
+}
+
+}  // namespace sihip
