@@ -16,18 +16,21 @@ __host__ __device__ inline uint32_t row_tiles(uint32_t tokens, uint32_t group) {
   return (tokens * group + 15u) / 16u;
 }
 
-// Shares that the rounds of all sequences are dealt to: the workgroups that
-// 256 CUs hold at once, over the kv heads and groups of row tiles; no more
-// than there can be rounds.
-constexpr uint32_t kCus = 256;
-inline uint32_t shares_for(const CacheView& c, uint32_t tile_groups, uint32_t per_cu,
-                           uint32_t round) {
+// Shares that the rounds of all sequences are dealt to: as many workgroups as
+// the card's 8 XCDs of 32 CUs hold at once, one a CU, over the kv heads.  The
+// groups of row tiles of one share and head go to one XCD; one workgroup more
+// than an XCD has CUs would wait for a whole share (verified drafts of three
+// groups: 113 us for 33 workgroups on some XCDs, 62 us for 30).  No more than
+// there can be rounds.
+constexpr uint32_t kXcds = 8, kXcdCus = 32;
+inline uint32_t shares_for(const CacheView& c, uint32_t tile_groups, uint32_t round) {
   const uint64_t rounds = (uint64_t)c.sequences * ((c.capacity + 31u) / round + 1u);
-  const uint32_t wanted = std::max(1u, kCus * per_cu / (c.kv_heads * tile_groups));
-  return (uint32_t)std::min<uint64_t>(wanted, rounds);
+  const uint32_t units = kXcds * std::max(1u, kXcdCus / tile_groups);
+  return (uint32_t)std::min<uint64_t>(std::max(1u, units / c.kv_heads), rounds);
 }
-// At most, whatever the kernel: two workgroups a CU.
-inline uint32_t shares_most(const CacheView& c) { return std::max(1u, 2u * kCus / c.kv_heads); }
+inline uint32_t shares_most(const CacheView& c) {
+  return std::max(1u, kXcds * kXcdCus / c.kv_heads);
+}
 
 // The workspace: (m, l) and the outputs before the division of the rows of
 // every (share, sequence) pair (Outputs); with weights (m, 1 / l) of every row
@@ -70,11 +73,13 @@ struct Outputs {
   float* scores;
   uint32_t score_stride, shares, tile_groups, round;
   float shift;  // p is held times 2^shift
+  bool q_vectors;  // the queries can be read in sixteen-byte pieces
+  Divisor by_group, by_heads, by_shares, by_tiles;  // group, kv_heads, shares, tile_groups
 };
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Maximum or sum over the lanes that share lane % 16: the second halves of the
+// Maximum over the lanes that share lane % 16: the second halves of the
 // wave, then its odd rows of 16, are put beside the first.
 __device__ __forceinline__ float columns_max(float v) {
   const uint32_t b = __float_as_uint(v);
@@ -96,18 +101,6 @@ __device__ __forceinline__ uint32_t slot_bits(uint32_t lo, uint32_t hi, uint32_t
 struct Span {
   uint32_t count, length, start, slots, rounds;
 };
-__device__ __forceinline__ Span span_of(const AttentionArgs& a, uint32_t seq, uint32_t round) {
-  Span s{brought(a.counts, seq, a.tokens), held(a.cache, seq), 0u, 0u, 1u};
-  if (s.count == 0u) return s;
-  uint32_t begin, end, other;
-  seen_slots(s.length, 0u, a.cache.capacity, a.window, begin, other);
-  seen_slots(s.length, s.count - 1u, a.cache.capacity, a.window, other, end);
-  s.start = begin / 32u * 32u;
-  s.slots = end > s.start ? end - s.start : 0u;
-  s.rounds = max(1u, (s.slots + round - 1u) / round);
-  return s;
-}
-
 // A value that all lanes hold, in a scalar register.
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -120,75 +113,113 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
   return v;
 }
 
-// All sequences' rounds, by a wave.
-__device__ __forceinline__ uint32_t all_rounds(const AttentionArgs& a, uint32_t round) {
-  const uint32_t lane = threadIdx.x & 63u, sequences = a.cache.sequences;
-  if (sequences == 1u) return span_of(a, 0u, round).rounds;
-  uint32_t total = 0u;
-  for (uint32_t base = lane; base < sequences; base += 64u) total += span_of(a, base, round).rounds;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-  return uniform(total);
-}
-
-// A workgroup's walk through the rounds of its share [at, end), `each` of them
-// or fewer: sequence `seq` has the rounds [first, first + rounds).
-struct Walk : Span {
-  uint32_t seq, first, at, end, each;
+// A workgroup's walk through its share of the rounds of all sequences, the
+// rounds [begin, limit) of [0, total).  Up to 64 sequences' lengths are read
+// once, a lane each.
+struct Walk {
+  uint32_t lengths, counts, upto;  // the lane's sequence, and the rounds up to its last
+  uint32_t begin, limit, at, end;  // the rounds that are left: [at, end)
+  uint32_t seq, first;             // the present sequence, its first round
+  Span span;
 };
-__device__ __forceinline__ void take(Walk& w, const Span& s) {
-  w.count = uniform(s.count), w.length = uniform(s.length), w.start = uniform(s.start);
-  w.slots = uniform(s.slots), w.rounds = uniform(s.rounds);
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, uint32_t count, uint32_t length,
+                                        uint32_t round) {
+  Span s{count, length, 0u, 0u, 1u};
+  if (count == 0u) return s;
+  uint32_t begin, end, other;
+  seen_slots(length, 0u, a.cache.capacity, a.window, begin, other);
+  seen_slots(length, count - 1u, a.cache.capacity, a.window, other, end);
+  s.start = begin & ~31u;
+  s.slots = end > s.start ? end - s.start : 0u;
+  s.rounds = max(1u, (s.slots + round - 1u) / round);
+  return s;
+}
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, uint32_t seq, uint32_t round) {
+  return span_of(a, brought(a.counts, seq, a.tokens), held(a.cache, seq), round);
 }
 
-// The walk's sequence: the one with round `w.at`.  Every lane of a wave takes part.
-__device__ __forceinline__ void find_sequence(const AttentionArgs& a, uint32_t round, Walk& w) {
-  const uint32_t lane = threadIdx.x & 63u, sequences = a.cache.sequences;
-  w.seq = w.first = 0u;
-  if (sequences == 1u) return take(w, span_of(a, 0u, round));
-  uint32_t before = 0u;
-  for (uint32_t base = 0; base < sequences; base += 64u) {
-    const uint32_t mine =
-        base + lane < sequences ? span_of(a, base + lane, round).rounds : 0u;
-    const uint32_t upto = wave_scan(mine, lane);
-    const uint64_t here = __builtin_amdgcn_ballot_w64(mine != 0u && w.at < before + upto);
-    if (here) {
-      const uint32_t at = (uint32_t)__builtin_ctzll(here);
-      w.seq = base + at;
-      w.first = before + __builtin_amdgcn_readlane(upto - mine, at);
-      return take(w, span_of(a, w.seq, round));
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
+// The present sequence's span.
+template <uint32_t ROUND>
+__device__ __forceinline__ void take_sequence(const AttentionArgs& a, Walk& w) {
+  uint32_t count, length;
+  if (a.cache.sequences <= 64u) {
+    count = __builtin_amdgcn_readlane(w.counts, w.seq);
+    length = __builtin_amdgcn_readlane(w.lengths, w.seq);
+  } else {
+    count = uniform(brought(a.counts, w.seq, a.tokens));
+    length = uniform(held(a.cache, w.seq));
   }
+  w.span = span_of(a, count, length, ROUND);
 }
-__device__ __forceinline__ Walk first_walk(const AttentionArgs& a, uint32_t round, uint32_t shares,
+template <uint32_t ROUND>
+__device__ __forceinline__ Walk first_walk(const AttentionArgs& a, const Outputs& o,
                                            uint32_t share) {
+  const uint32_t lane = threadIdx.x & 63u, sequences = a.cache.sequences;
   Walk w{};
-  const uint32_t total = all_rounds(a, round);
-  w.each = uniform((total + shares - 1u) / shares);
-  const uint64_t at = (uint64_t)share * w.each;
-  w.at = uniform((uint32_t)min(at, (uint64_t)total));
-  w.end = uniform((uint32_t)min(at + w.each, (uint64_t)total));
-  if (w.at < w.end) find_sequence(a, round, w);
+  uint32_t total = 0u;
+  for (uint32_t base = 0; base < sequences; base += 64u) {
+    uint32_t rounds = 0u;
+    if (base + lane < sequences) {
+      w.counts = brought(a.counts, base + lane, a.tokens);
+      w.lengths = held(a.cache, base + lane);
+      rounds = span_of(a, w.counts, w.lengths, ROUND).rounds;
+    }
+    w.upto = total + wave_scan(rounds, lane);
+    total = __builtin_amdgcn_readlane(w.upto, 63);
+  }
+  const uint32_t each = o.by_shares.of(total + o.shares - 1u);
+  w.begin = w.at = min(share * each, total);
+  w.end = min(w.begin + each, total);
+  w.limit = w.begin + each;
+  if (w.at >= w.end) return w;
+  if (sequences <= 64u) {
+    w.seq = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(w.at < w.upto));
+  } else {  // the first whose last round is not before `at`
+    uint32_t before = 0u;
+    for (uint32_t base = 0;; base += 64u) {
+      const uint32_t rounds = base + lane < sequences ? span_of(a, base + lane, ROUND).rounds : 0u;
+      const uint32_t upto = before + wave_scan(rounds, lane);
+      const uint64_t here = __builtin_amdgcn_ballot_w64(w.at < upto);
+      if (here) {
+        const uint32_t at = (uint32_t)__builtin_ctzll(here);
+        w.seq = base + at;
+        w.first = __builtin_amdgcn_readlane(upto - rounds, at);
+        break;
+      }
+      before = __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  take_sequence<ROUND>(a, w);
+  if (sequences <= 64u) w.first = __builtin_amdgcn_readlane(w.upto, w.seq) - w.span.rounds;
   return w;
 }
-__device__ __forceinline__ void next_walk(const AttentionArgs& a, uint32_t round, Walk& w) {
-  w.at = w.first = w.first + w.rounds;
+template <uint32_t ROUND>
+__device__ __forceinline__ void next_sequence(const AttentionArgs& a, Walk& w) {
+  w.at = w.first = w.first + w.span.rounds;
   if (w.at >= w.end) return;
   ++w.seq;
-  take(w, span_of(a, w.seq, round));
+  take_sequence<ROUND>(a, w);
 }
 
 // ---- running maxima and sums -------------------------------------------------------
-// (m, l) of two sets of a row's slots, joined.  l < 0: there are slots, and all
-// scores are -inf, which says nothing beside a set that has others.
-__device__ __forceinline__ float2 joined(float2 x, float2 y) {
-  const float m = fmaxf(x.x, y.x);
-  const float u = x.x == -INFINITY ? (x.y < 0.0f ? 0.0f : x.y) : x.y * exp2_of(x.x - m);
-  const float v = y.x == -INFINITY ? (y.y < 0.0f ? 0.0f : y.y) : y.y * exp2_of(y.x - m);
-  const bool no_more = m == -INFINITY && (x.y < 0.0f || y.y < 0.0f) && u + v == 0.0f;
-  return make_float2(m, no_more ? -1.0f : u + v);
-}
+// (m, l) of sets of a row's slots, joined to those of all of them.  l < 0: there
+// are slots, and all scores are -inf, which says nothing beside a set that has
+// others.  A set's sum is taken times 2^(its m - the joint one).
+struct Joined {
+  float m = -INFINITY, l = 0.0f;
+  bool minus = false;
+  __device__ __forceinline__ static float times(float m, float top) {
+    return m == -INFINITY ? 1.0f : exp2_of(m - top);  // (l is 0, -1 or no number)
+  }
+  // with `top` the joint maximum
+  __device__ __forceinline__ void add(float2 set, float top) {
+    minus |= set.y < 0.0f;
+    l = fmaf(set.y < 0.0f ? 0.0f : set.y, times(set.x, top), l);
+  }
+  __device__ __forceinline__ float2 result(float top) const {
+    return make_float2(top, minus && top == -INFINITY && l == 0.0f ? -1.0f : l);
+  }
+};
 // What a row's sums are taken times in the end, and its (m, 1 / l) for the
 // weights: 0 / 0 where every score is -inf.
 __device__ __forceinline__ float row_times(float2 st) {

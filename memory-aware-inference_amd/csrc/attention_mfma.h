@@ -21,7 +21,12 @@
 // half loses bits to F16's range.  An f32 cache takes the f32 instructions.
 // Products and sums are f32.
 //
-// The slots of all sequences, in rounds of one tile for each wave of a
+// A wave has up to 128 values of a head.  Of a larger one two waves take a half
+// each, of the keys and of the values: they add their halves' scores through
+// LDS, and both go on with the sums.  The queries of one row tile stay in
+// registers; those of several are in LDS.
+//
+// The slots of all sequences, in rounds of one tile for each team of waves of a
 // workgroup, are dealt to the workgroups of a kv head in equal shares, one
 // after another: a share may end one sequence and begin others.  A sequence
 // inside one share is written at once; the sums of one that lies in several
@@ -92,23 +97,38 @@ struct F32 {
   static constexpr uint32_t kExponent = 0x7f800000u, kUnit = 0x00800000u, kCarry = 0x80000000u;
 };
 
-template <typename T, uint32_t DC, uint32_t RT, uint32_t WAVES>
+// DW: values of a head that a wave has; VS: waves of a team, which have a head
+// together; RT: row tiles a wave.
+template <typename T, uint32_t DW, uint32_t VS, uint32_t RT>
 struct Shape {
+  static constexpr uint32_t kWaves = 8, kTeams = kWaves / VS;
   static constexpr bool kWide = T::kBytes == 4;               // f32 instructions
   static constexpr uint32_t kSubs = T::kSlots / 16;           // score tiles of 16 slots
-  static constexpr uint32_t kSteps = DC / (kWide ? 16 : 32);  // 16-byte pieces of a key a lane
+  static constexpr uint32_t kSteps = DW / (kWide ? 16 : 32);  // 16-byte pieces of a key a lane
+  static constexpr uint32_t kValues = kWide ? 4 : 8;          // values of such a piece
   static constexpr uint32_t kRows = kWide ? 4 : 8;            // value rows a lane
   // values of a row that a lane loads at once, and how often
-  static constexpr uint32_t kEach = kWide ? 4 : DC >= 128 ? 8 : 4;
-  static constexpr uint32_t kPasses = DC / (16 * kEach);
+  static constexpr uint32_t kEach = kWide ? 4 : DW >= 128 ? 8 : 4;
+  static constexpr uint32_t kPasses = DW / (16 * kEach);
   static constexpr uint32_t kWords = kEach * T::kBytes / 4;
-  static constexpr uint32_t kTiles = DC / 16;  // of the output
-  static constexpr uint32_t kItems = RT * kSteps * 64;  // 16-byte pieces of the queries
-  static constexpr uint32_t kQueryBytes = T::kPieces * kItems * 16;
-  static constexpr uint32_t kOutStride = DC + 4;  // words of a row of the join
-  static constexpr uint32_t kOutBytes = WAVES / 2 * 16 * kOutStride * 4;  // half the waves'
-  static constexpr uint32_t kShared = kQueryBytes > kOutBytes ? kQueryBytes : kOutBytes;
+  static constexpr uint32_t kTiles = DW / 16;  // of the wave's output
+  static constexpr bool kInRegisters = RT == 1;  // the queries
+  static constexpr uint32_t kItems = VS * RT * kSteps * 64;  // 16-byte pieces of the queries
+  static constexpr uint32_t kQueryBytes = kInRegisters ? 0 : T::kPieces * kItems * 16;
+  // halves of scores that the waves of a team exchange
+  static constexpr uint32_t kBuffers = VS == 1 ? 0 : RT > 2 ? 1 : 2;
+  static constexpr uint32_t kExchange = kWaves * RT * kSubs * 64 * 16;
+  static constexpr uint32_t kOutStride = DW * VS + 4;  // words of a row of the join
+  static constexpr uint32_t kOutBytes = kTeams * 16 * kOutStride * 4;
+  static constexpr uint32_t kTileBytes = kQueryBytes + kBuffers * kExchange;
+  static constexpr uint32_t kShared = kTileBytes > kOutBytes ? kTileBytes : kOutBytes;
 };
+
+// The workgroup's waves meet, what they wrote to LDS in place.  Loads from
+// memory go on.
+__device__ __forceinline__ void exchange_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
 // Blocks of the row tiles of one share and head follow each other on one XCD
 // (blocks are dealt to the eight in turn), so its L2 serves them the same rows.
@@ -119,22 +139,24 @@ __device__ __forceinline__ void block_work(const Outputs& o, uint32_t& unit, uin
     tile = 0u;
     return;
   }
-  const uint32_t xcd = b & 7u, i = b >> 3, row = uniform(i / o.tile_groups);
+  const uint32_t xcd = b & 7u, i = b >> 3, row = o.by_tiles.of(i);
   tile = i - row * o.tile_groups;
   unit = row * 8u + xcd;
 }
 
-template <typename T, uint32_t DC, bool FULL, uint32_t RT, uint32_t WAVES, uint32_t PER_SIMD>
-__global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(AttentionArgs a, Outputs o) {
-  using S = Shape<T, DC, RT, WAVES>;
-  constexpr uint32_t kThreads = 64 * WAVES, kRound = T::kSlots * WAVES;
+// FAST: heads of DW * VS values on pages of whole sixteens of slots, so that the
+// slots of a score tile lie one after another and addresses are scalars.
+template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT>
+__global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Outputs o) {
+  using S = Shape<T, DW, VS, RT>;
+  constexpr uint32_t kThreads = 64 * S::kWaves, kRound = T::kSlots * S::kTeams;
   extern __shared__ __attribute__((aligned(16))) uint8_t shared[];
-  __shared__ float row_m[WAVES][RT * 16], row_l[WAVES][RT * 16];
+  __shared__ float row_m[S::kTeams][RT * 16], row_l[S::kTeams][RT * 16];
+  __shared__ float2 row_sum[RT * 16];
   __shared__ uint32_t row_top[RT * 16];
-  __shared__ uint32_t last_share;
   const CacheView& c = a.cache;
-  const uint32_t wave = uniform(threadIdx.x / 64u);
-  const uint32_t dim = FULL ? DC : c.head_dim;
+  const uint32_t wave = uniform(threadIdx.x / 64u), team = wave / VS, half = wave % VS;
+  const uint32_t dim = FAST ? DW * VS : c.head_dim;
   const uint32_t row_bytes = dim * T::kBytes;
   const uint32_t rows = a.tokens * a.group;
   const uint8_t* keys = static_cast<const uint8_t*>(c.keys);
@@ -144,9 +166,9 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
   uint32_t unit, group_at;
   block_work(o, unit, group_at);
   if (unit >= o.shares * c.kv_heads) return;
-  const uint32_t share = uniform(unit / c.kv_heads), kv = unit - share * c.kv_heads;
+  const uint32_t share = o.by_heads.of(unit), kv = unit - share * c.kv_heads;
   const uint32_t row0 = group_at * (RT * 16u);
-  Walk walk = first_walk(a, kRound, o.shares, share);
+  Walk walk = first_walk<kRound>(a, o, share);
 
   while (walk.at < walk.end) {
   // (afresh for each sequence: what follows from the thread's number would
@@ -154,71 +176,109 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
   uint32_t tid = threadIdx.x;
   asm volatile("" : "+v"(tid));
   const uint32_t lane = tid & 63u, n = lane & 15u, j = lane >> 4;
-  const uint32_t seq = walk.seq;
-  const uint32_t count = walk.count, length = walk.length;
-  const uint32_t c0 = walk.start + (walk.at - walk.first) * kRound;
-  const uint32_t c1 = min(c0 + (min(walk.end, walk.first + walk.rounds) - walk.at) * kRound,
-                          walk.start + walk.slots);
+  const uint32_t seq = walk.seq, count = walk.span.count, length = walk.span.length;
+  const uint32_t c0 = walk.span.start + (walk.at - walk.first) * kRound;
+  const uint32_t c1 = min(c0 + (min(walk.end, walk.first + walk.span.rounds) - walk.at) * kRound,
+                          walk.span.start + walk.span.slots);
+  // the sequence lies in this share
+  const bool alone = walk.first >= walk.begin && walk.first + walk.span.rounds <= walk.limit;
+
   if (kv == 0u && group_at == 0u && walk.at == walk.first && tid == 0u && count != 0u &&
       (uint64_t)c.lengths[seq] + count > c.capacity)
     report_device_error(a.report, kDevErrCacheFull);
 
   // ---- the slots that the rows see: any of them, and all
-  const uint32_t t_first = min(uniform(row0 / a.group), count);
-  const uint32_t t_last = min(uniform((min(row0 + RT * 16u, rows) - 1u) / a.group) + 1u, count);
+  const uint32_t t_first = min(o.by_group.of(row0), count);
+  const uint32_t t_last = min(o.by_group.of(min(row0 + RT * 16u, rows) - 1u) + 1u, count);
   uint32_t any_lo = 0u, any_hi = 0u, all_lo = 0u, all_hi = 0u;
   if (t_first < t_last) {
     seen_slots(length, t_first, c.capacity, a.window, any_lo, all_hi);
     seen_slots(length, t_last - 1u, c.capacity, a.window, all_lo, any_hi);
   }
   const uint32_t hi = min(c1, any_hi);
-  const uint32_t first = c0 + wave * T::kSlots;
+  const uint32_t first = c0 + team * T::kSlots;
 
-  // A tile's rows in two steps, so that the page numbers are there before the
-  // rows are wanted: lane l has slot l % kSlots.
-  const auto page_of = [&](uint32_t base) {
-    const uint32_t slot = base + (lane & (T::kSlots - 1u));
-    return slot < hi ? c.table[(size_t)seq * c.max_pages + divided(slot, c.div_mul, c.div_shift)]
-                     : kNone;
+  // Where a tile's rows lie, in two steps, so that the page numbers are there
+  // before the rows are wanted.  FAST: of each score tile; else lane l has slot
+  // l % kSlots.
+  struct Place {
+    uint32_t at[FAST ? S::kSubs : 1];
   };
+  const uint32_t* table = c.table + (size_t)seq * c.max_pages;
   uint32_t bad = 0u;
-  const auto row_of = [&](uint32_t base, uint32_t page) {
-    const uint32_t slot = base + (lane & (T::kSlots - 1u));
-    if (slot >= hi) return kNone;
-    if (page >= c.pages) {
-      bad = 1u;
-      return kNone;
+  const auto pages_of = [&](uint32_t base) {
+    Place p;
+    if constexpr (FAST) {
+#pragma unroll
+      for (uint32_t s = 0; s < S::kSubs; ++s) {
+        const uint32_t slot = base + s * 16u;
+        p.at[s] = slot < hi ? table[divided(slot, c.div_mul, c.div_shift)] : kNone;
+      }
+    } else {
+      const uint32_t slot = base + (lane & (T::kSlots - 1u));
+      p.at[0] = slot < hi ? table[divided(slot, c.div_mul, c.div_shift)] : kNone;
     }
-    return (page * c.kv_heads + kv) * c.page_tokens +
-           (slot - divided(slot, c.div_mul, c.div_shift) * c.page_tokens);
+    return p;
   };
-  // (a slot without a row reads the pool's first one, and is masked)
-  const auto pointer = [&](const uint8_t* base, uint32_t row, uint32_t from) {
-    const uint32_t at = __shfl(row, from, 64);
-    return base + (size_t)(at == kNone ? 0u : at) * row_bytes;
+  const auto rows_of = [&](uint32_t base, const Place& page) {
+    Place p;
+#pragma unroll
+    for (uint32_t s = 0; s < (FAST ? S::kSubs : 1u); ++s) {
+      const uint32_t slot = base + (FAST ? s * 16u : lane & (T::kSlots - 1u));
+      p.at[s] = kNone;
+      if (slot < hi) {
+        if (page.at[s] < c.pages)
+          p.at[s] = (page.at[s] * c.kv_heads + kv) * c.page_tokens +
+                    (slot - divided(slot, c.div_mul, c.div_shift) * c.page_tokens);
+        else
+          bad = 1u;
+      }
+    }
+    return p;
+  };
+  // The slots that have a row, a bit each.  (FAST: and those behind the last
+  // on its page, which no row of the queries sees.)
+  const auto slots_there = [&](const Place& p) {
+    if constexpr (!FAST) return (uint32_t)__builtin_amdgcn_ballot_w64(p.at[0] != kNone);
+    uint32_t bits = 0u;
+#pragma unroll
+    for (uint32_t s = 0; s < (FAST ? S::kSubs : 1u); ++s)
+      bits |= p.at[s] != kNone ? 0xffffu << (16u * s) : 0u;
+    return bits;
+  };
+  // Row `from` of score tile `sub`; a slot without a row reads the pool's first
+  // page, or first row, and is masked.
+  const auto pointer = [&](const uint8_t* base, const Place& p, uint32_t sub, uint32_t from) {
+    if constexpr (FAST) {
+      const uint32_t at = p.at[sub];
+      return base + (size_t)(at == kNone ? 0u : at) * row_bytes + from * row_bytes;
+    } else {
+      const uint32_t at = __shfl(p.at[0], sub * 16u + from, 64);
+      return base + (size_t)(at == kNone ? 0u : at) * row_bytes;
+    }
   };
   u32x4 key[S::kSubs][S::kSteps];
-  const auto load_keys = [&](uint32_t row) {
+  const auto load_keys = [&](const Place& row) {
 #pragma unroll
     for (uint32_t s = 0; s < S::kSubs; ++s) {
-      const uint8_t* p = pointer(keys, row, s * 16u + n);
+      const uint8_t* p = pointer(keys, row, s, n);
 #pragma unroll
       for (uint32_t k = 0; k < S::kSteps; ++k) {
-        uint32_t at = (k * 4u + j) * 16u;
-        if (!FULL) at = min(at, row_bytes - 16u);  // (its query values are 0)
+        uint32_t at = ((half * S::kSteps + k) * 4u + j) * 16u;
+        if (!FAST) at = min(at, row_bytes - 16u);  // (its query values are 0)
         key[s][k] = *reinterpret_cast<const u32x4*>(p + at);
       }
     }
   };
   uint32_t value[S::kRows][S::kPasses][S::kWords];
-  const auto load_values = [&](uint32_t row) {
+  const auto load_values = [&](const Place& row) {
 #pragma unroll
     for (uint32_t i = 0; i < S::kRows; ++i) {
-      const uint8_t* p = pointer(values, row, i / 4u * 16u + j * 4u + i % 4u);
+      const uint8_t* p = pointer(values, row, i / 4u, j * 4u + i % 4u);
 #pragma unroll
       for (uint32_t u = 0; u < S::kPasses; ++u) {
-        uint32_t at = (u * 16u + n) * (S::kWords * 4u);
-        if (!FULL) at = min(at, row_bytes - S::kWords * 4u);  // (its outputs are not stored)
+        uint32_t at = ((half * S::kPasses + u) * 16u + n) * (S::kWords * 4u);
+        if (!FAST) at = min(at, row_bytes - S::kWords * 4u);  // (its outputs are not stored)
         if constexpr (S::kWords == 4) {
           const u32x4 w = *reinterpret_cast<const u32x4*>(p + at);
 #pragma unroll
@@ -232,66 +292,84 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
     }
   };
 
-  // ---- the rows' queries, as B operands, into LDS; the first keys are under
-  // way meanwhile (loads return in order, so the queries' go first)
-  uint32_t page = page_of(first);
-  uint32_t next_page = page_of(first + kRound);
-  constexpr uint32_t kValues = S::kWide ? 4 : 8;
-  constexpr uint32_t kMine = (S::kItems + kThreads - 1) / kThreads;
-  float x[kMine][kValues];
+  // ---- the rows' queries, as B operands; the first keys are under way meanwhile
+  // (loads return in order, so the queries' go first)
+  Place page = pages_of(first), next_page = pages_of(first + kRound);
   const float scale = a.scale * kLog2e;
+  // Sixteen-byte pieces of the operands: those of the wave's half where they
+  // stay in registers, else the thread's share of all.
+  constexpr uint32_t kMine = S::kInRegisters ? S::kSteps : (S::kItems + kThreads - 1) / kThreads;
+  const auto item = [&](uint32_t k) {  // row tile, half, step, lane: the piece's place in LDS
+    return S::kInRegisters ? (half * S::kSteps + k) * 64u + lane : tid + k * kThreads;
+  };
+  const auto item_row = [&](uint32_t i) { return i / (VS * S::kSteps * 64u) * 16u + (i & 15u); };
+  float x[kMine][S::kValues];
 #pragma unroll
   for (uint32_t k = 0; k < kMine; ++k) {
-    const uint32_t i = tid + k * kThreads, l = i & 63u;
-    const uint32_t r = row0 + i / (S::kSteps * 64u) * 16u + (l & 15u), t = r / a.group;
-    const uint32_t d0 = (i / 64u % S::kSteps * 4u + (l >> 4)) * kValues;
+    const uint32_t i = item(k), r = row0 + item_row(i), t = o.by_group.of(r);
+    const uint32_t d0 = (i / 64u % (VS * S::kSteps) * 4u + ((i & 63u) >> 4)) * S::kValues;
     const bool there = i < S::kItems && r < rows && t < count && d0 < dim;
     const float* src = a.q + ((size_t)seq * a.tokens + t) * a.q_token_stride +
                        (kv * a.group + (r - t * a.group)) * a.q_head_stride + d0;
+    if (o.q_vectors) {
 #pragma unroll
-    for (uint32_t v = 0; v < kValues; ++v) x[k][v] = there ? src[v] : 0.0f;
+      for (uint32_t v = 0; v < S::kValues; v += 4) {
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (there) f = *reinterpret_cast<const float4*>(src + v);
+        x[k][v] = f.x, x[k][v + 1] = f.y, x[k][v + 2] = f.z, x[k][v + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (uint32_t v = 0; v < S::kValues; ++v) x[k][v] = there ? src[v] : 0.0f;
+    }
   }
-  uint32_t row = row_of(first, page);
+  Place row = rows_of(first, page);
   load_keys(row);
   page = next_page;
-  if constexpr (T::kShift != 0.0f) {
+  // The largest of a row's values, as an integer (what is no number is larger
+  // than all): in LDS, or of the wave's half over the lanes that have it.
+  uint32_t largest = 0u;
+  if (!S::kInRegisters && T::kShift != 0.0f) {
     if (tid < RT * 16u) row_top[tid] = 0u;
     __syncthreads();
   }
 #pragma unroll
   for (uint32_t k = 0; k < kMine; ++k) {
-    float top = 0.0f;
+    uint32_t top = 0u;
 #pragma unroll
-    for (uint32_t v = 0; v < kValues; ++v) {
+    for (uint32_t v = 0; v < S::kValues; ++v) {
       x[k][v] *= scale;
-      // (as integers, what is no number is the largest of them)
-      if (T::kShift != 0.0f)
-        top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(x[k][v]) & 0x7fffffffu));
+      top = max(top, __float_as_uint(x[k][v]) & 0x7fffffffu);
     }
-    if constexpr (T::kShift != 0.0f) {
-      const uint32_t i = tid + k * kThreads;
-      if (i < S::kItems)
-        atomicMax(&row_top[i / (S::kSteps * 64u) * 16u + (i & 15u)], __float_as_uint(top));
+    if (T::kShift != 0.0f) {
+      if (S::kInRegisters) largest = max(largest, top);
+      else if (item(k) < S::kItems) atomicMax(&row_top[item_row(item(k))], top);
     }
   }
-  // the rows' powers of two, 2^14 at the largest value; 1 where it is no number
+  if (T::kShift != 0.0f) {
+    if (S::kInRegisters) {
+      largest = max(largest, (uint32_t)__shfl_xor(largest, 16, 64));
+      largest = max(largest, (uint32_t)__shfl_xor(largest, 32, 64));
+    } else {
+      __syncthreads();
+    }
+  }
+  // the row's power of two, 2^14 at the largest value; 1 where that is no number
   const auto power = [&](uint32_t r) {
-    const uint32_t e = row_top[r] >> 23;
+    const uint32_t e = (S::kInRegisters ? largest : row_top[r]) >> 23;
     return e == 255u ? 1.0f : __uint_as_float((268u - max(e, 16u)) << 23);
   };
-  if constexpr (T::kShift != 0.0f) __syncthreads();
+  u32x4 query[S::kInRegisters ? S::kSteps : 1][T::kPieces];
 #pragma unroll
   for (uint32_t k = 0; k < kMine; ++k) {
-    const uint32_t i = tid + k * kThreads;
+    const uint32_t i = item(k);
     if (i >= S::kItems) break;
+    u32x4 w[T::kPieces];
     if constexpr (S::kWide) {
-      u32x4 w;
 #pragma unroll
-      for (uint32_t v = 0; v < 4; ++v) w[v] = __float_as_uint(x[k][v]);
-      q_lds[i] = w;
+      for (uint32_t v = 0; v < 4; ++v) w[0][v] = __float_as_uint(x[k][v]);
     } else {
-      u32x4 w[T::kPieces];
-      const float s = T::kShift != 0.0f ? power(i / (S::kSteps * 64u) * 16u + (i & 15u)) : 1.0f;
+      const float s = T::kShift != 0.0f ? power(item_row(i)) : 1.0f;
 #pragma unroll
       for (uint32_t v = 0; v < 8; v += 2) {
         uint32_t p[T::kPieces];
@@ -299,11 +377,15 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
 #pragma unroll
         for (uint32_t q = 0; q < T::kPieces; ++q) w[q][v / 2] = p[q];
       }
+    }
 #pragma unroll
-      for (uint32_t q = 0; q < T::kPieces; ++q) q_lds[q * S::kItems + i] = w[q];
+    for (uint32_t q = 0; q < T::kPieces; ++q) {
+      if constexpr (S::kInRegisters) query[k][q] = w[q];
+      else q_lds[q * S::kItems + i] = w[q];
     }
   }
-  __syncthreads();
+  if (!S::kInRegisters) __syncthreads();
+  load_values(row);
 
   // ---- the lane's rows, and their slots
   uint32_t begin[RT], end[RT];
@@ -313,7 +395,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
   f32x4 out[RT][S::kTiles];
 #pragma unroll
   for (uint32_t i = 0; i < RT; ++i) {
-    const uint32_t r = row0 + i * 16u + n, t = r / a.group;
+    const uint32_t r = row0 + i * 16u + n, t = o.by_group.of(r);
     begin[i] = end[i] = 0u;
     score_row[i] = nullptr;
     if (r < rows && t < count) {
@@ -354,80 +436,115 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
 #pragma unroll
           for (uint32_t k = 0; k < T::kPieces; ++k) b[r][k][i / 2] = w[k];
         }
+      // (four sums at a time, so that none waits for the one before)
 #pragma unroll
       for (uint32_t u = 0; u < S::kPasses; ++u)
 #pragma unroll
-        for (uint32_t d = 0; d < S::kEach; ++d) {
-          u32x4 v;
+        for (uint32_t d = 0; d < S::kEach; d += 4) {
+          u32x4 v[4];
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i)
-            v[i] = perm(value[2 * i + 1][u][d / 2], value[2 * i][u][d / 2], d & 1 ? kHighs : kLows);
+          for (uint32_t e = 0; e < 4; ++e)
 #pragma unroll
-          for (uint32_t k = 0; k < T::kPieces; ++k)
+            for (uint32_t i = 0; i < 4; ++i)
+              v[e][i] = perm(value[2 * i + 1][u][(d + e) / 2], value[2 * i][u][(d + e) / 2],
+                             e & 1 ? kHighs : kLows);
 #pragma unroll
-            for (uint32_t r = 0; r < RT; ++r)
-              out[r][u * S::kEach + d] = T::mfma(v, b[r][k], out[r][u * S::kEach + d]);
+          for (uint32_t r = 0; r < RT; ++r)
+#pragma unroll
+            for (uint32_t k = 0; k < T::kPieces; ++k)
+#pragma unroll
+              for (uint32_t e = 0; e < 4; ++e) {
+                f32x4& acc = out[r][u * S::kEach + d + e];
+                acc = T::mfma(v[e], b[r][k], acc);
+              }
         }
     }
   };
 
-  for (uint32_t base = first; base < hi; base += kRound) {
-    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(row != kNone);
-    next_page = page_of(base + 2u * kRound);
-    load_values(row);
-    __builtin_amdgcn_sched_barrier(0);
+  // (a team without slots in the last round goes through it: its waves, and the
+  // others', meet at the exchange)
+  uint32_t turn = 0u;
+  for (uint32_t at = c0; at < hi; at += kRound) {
+    const uint32_t base = at + team * T::kSlots;
+    const uint32_t there = slots_there(row);
+    next_page = pages_of(base + 2u * kRound);
     // ---- scores
-    // (the queries are read each time: kept across tiles, they would not leave registers for
-    // the tile)
-    uint32_t q_at = lane;
-    asm volatile("" : "+v"(q_at));
     f32x4 sum[RT][S::kSubs];
+    // (queries in LDS are read for each tile: kept across tiles, they would not leave
+    // registers for it; a step's are under way while the one before is multiplied)
+    uint32_t q_at = half * S::kSteps * 64u + lane;
+    asm volatile("" : "+v"(q_at));
+    const auto read_query = [&](uint32_t i, u32x4(&q)[T::kPieces]) {
+      if constexpr (!S::kInRegisters)
+#pragma unroll
+        for (uint32_t w = 0; w < T::kPieces; ++w)
+          q[w] = q_lds[w * S::kItems + (i / S::kSteps * VS * S::kSteps + i % S::kSteps) * 64u + q_at];
+      else
+#pragma unroll
+        for (uint32_t w = 0; w < T::kPieces; ++w) q[w] = query[i][w];
+    };
+    u32x4 q[2][T::kPieces];
+    read_query(0u, q[0]);
 #pragma unroll
     for (uint32_t r = 0; r < RT; ++r) {
-      if constexpr (S::kWide) {
-        f32x4 even{0, 0, 0, 0}, odd{0, 0, 0, 0};
+      // sums that do not wait for each other: two of the f32 instructions, one a piece else
+      constexpr uint32_t kSums = S::kWide ? 2 : T::kPieces;
+      f32x4 piece[S::kSubs][kSums];
 #pragma unroll
-        for (uint32_t k = 0; k < S::kSteps; ++k) {
-          const u32x4 q = q_lds[(r * S::kSteps + k) * 64u + q_at];
+      for (uint32_t s = 0; s < S::kSubs; ++s)
 #pragma unroll
-          for (uint32_t e = 0; e < 4; e += 2) {
-            even = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(key[0][k][e]),
-                                                        __uint_as_float(q[e]), even, 0, 0, 0);
-            odd = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(key[0][k][e + 1]),
-                                                       __uint_as_float(q[e + 1]), odd, 0, 0, 0);
-          }
-        }
-        sum[r][0] = even + odd;
-      } else {
-        f32x4 piece[S::kSubs][T::kPieces];
+        for (uint32_t k = 0; k < kSums; ++k) piece[s][k] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t s = 0; s < S::kSubs; ++s)
+      for (uint32_t k = 0; k < S::kSteps; ++k) {
+        const uint32_t i = r * S::kSteps + k;
+        if (i + 1u < RT * S::kSteps) read_query(i + 1u, q[(i + 1u) & 1u]);
+        if (!S::kInRegisters) __builtin_amdgcn_sched_barrier(0);
+        const auto& now = q[i & 1u];
+        if constexpr (S::kWide) {
 #pragma unroll
-          for (uint32_t k = 0; k < T::kPieces; ++k) piece[s][k] = f32x4{0, 0, 0, 0};
+          for (uint32_t e = 0; e < 4; ++e)
+            piece[0][e & 1u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                __uint_as_float(key[0][k][e]), __uint_as_float(now[0][e]), piece[0][e & 1u], 0, 0, 0);
+        } else {
 #pragma unroll
-        for (uint32_t k = 0; k < S::kSteps; ++k)
-#pragma unroll
-          for (uint32_t w = 0; w < T::kPieces; ++w) {
-            const u32x4 q = q_lds[w * S::kItems + (r * S::kSteps + k) * 64u + q_at];
+          for (uint32_t w = 0; w < T::kPieces; ++w)
 #pragma unroll
             for (uint32_t s = 0; s < S::kSubs; ++s)
-              piece[s][w] = T::mfma(key[s][k], q, piece[s][w]);
-          }
-#pragma unroll
-        for (uint32_t s = 0; s < S::kSubs; ++s) {
-          sum[r][s] = piece[s][T::kPieces - 1];
-#pragma unroll
-          for (int k = (int)T::kPieces - 2; k >= 0; --k) sum[r][s] += piece[s][k];
-          sum[r][s] *= unscale[r];
+              piece[s][w] = T::mfma(key[s][k], now[w], piece[s][w]);
         }
+      }
+#pragma unroll
+      for (uint32_t s = 0; s < S::kSubs; ++s) {
+        sum[r][s] = piece[s][kSums - 1];
+#pragma unroll
+        for (int k = (int)kSums - 2; k >= 0; --k) sum[r][s] += piece[s][k];
+        if (T::kShift != 0.0f) sum[r][s] *= unscale[r];
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     // ---- the next tile's keys
-    row = row_of(base + kRound, page);
+    row = rows_of(base + kRound, page);
     page = next_page;
     load_keys(row);  // (behind the last tile too: a condition would hold both sets of registers)
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (VS == 2) {
+      // ---- the other half's scores: both waves add the first half's to the second's
+      f32x4* place = reinterpret_cast<f32x4*>(shared + S::kQueryBytes) +
+                     (turn % S::kBuffers) * (S::kExchange / 16u);
+      if (S::kBuffers == 1u) exchange_barrier();  // (the last ones are taken)
+#pragma unroll
+      for (uint32_t r = 0; r < RT; ++r)
+#pragma unroll
+        for (uint32_t s = 0; s < S::kSubs; ++s)
+          place[((wave * RT + r) * S::kSubs + s) * 64u + lane] = sum[r][s];
+      exchange_barrier();
+#pragma unroll
+      for (uint32_t r = 0; r < RT; ++r)
+#pragma unroll
+        for (uint32_t s = 0; s < S::kSubs; ++s)
+          sum[r][s] += place[(((wave ^ 1u) * RT + r) * S::kSubs + s) * 64u + lane];
+      ++turn;
+    }
     // ---- p
     float p[RT][S::kRows];
     uint32_t seen[RT];  // bits 0..3 and 16..19: the row sees the lane's slots
@@ -442,7 +559,7 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
         top = fmaxf(top, p[r][i]);
       }
       any |= seen[r] ? 1u << r : 0u;
-      if (score_row[r]) {
+      if (score_row[r] && half == 0u) {
 #pragma unroll
         for (uint32_t s = 0; s < S::kSubs; ++s) {
           const uint32_t slot = base + s * 16u + j * 4u;
@@ -509,6 +626,8 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
       }
     }
     add_values(p);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(row);  // the next tile's
   }
   if (bad) report_device_error(a.report, kDevErrCachePage);
 
@@ -522,70 +641,57 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
     if (l[r] == 0.0f && m[r] == -INFINITY && (any >> r & 1u) != 0u) l[r] = -1.0f;
-    if (j == 0u) {
-      row_m[wave][r * 16u + n] = m[r];
-      row_l[wave][r * 16u + n] = l[r];
+    if (j == 0u && half == 0u) {
+      row_m[team][r * 16u + n] = m[r];
+      row_l[team][r * 16u + n] = l[r];
     }
   }
-  // the sequence's shares, and this one among them
-  const uint32_t shares =
-      uniform((walk.first + walk.rounds - 1u) / walk.each) - uniform(walk.first / walk.each) + 1u;
-  float* join = reinterpret_cast<float*>(shared) + ((wave % (WAVES / 2u)) * 16u + n) * S::kOutStride;
-  const auto place = [&](uint32_t u, uint32_t w) {
-    return reinterpret_cast<float4*>(join + (u * 16u + j * 4u + w) * S::kEach);
-  };
+  float* join = reinterpret_cast<float*>(shared) + (team * 16u + n) * S::kOutStride;
 #pragma unroll
   for (uint32_t r = 0; r < RT; ++r) {
-    __syncthreads();  // (the queries, or the last tile's outputs, are no longer read)
+    __syncthreads();  // (the queries and scores, or the last tile's outputs, are no longer read)
     float top = -INFINITY;
 #pragma unroll
-    for (uint32_t w = 0; w < WAVES; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
-    const float mine = m[r] == -INFINITY ? 0.0f : exp2_of(m[r] - top);
+    for (uint32_t w = 0; w < S::kTeams; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
+    if (wave == 0u) {
+      Joined sum_l;
 #pragma unroll
-    for (uint32_t d = 0; d < S::kTiles; ++d) out[r][d] *= mine;
-    // the second half of the waves hands its outputs to the first, which hands its sums to all
-#pragma unroll
-    for (uint32_t half = 0; half < 2; ++half) {
-      if ((wave >= WAVES / 2u) == (half == 0u)) {
-#pragma unroll
-        for (uint32_t u = 0; u < S::kPasses; ++u)
-#pragma unroll
-          for (uint32_t w = 0; w < 4; ++w)
-#pragma unroll
-            for (uint32_t d = 0; d < S::kEach; d += 4) {
-              f32x4* t = &out[r][u * S::kEach + d];
-              float4* to = place(u, w) + d / 4u;
-              if (half == 1u) {
-                const float4 v = *to;
-                t[0][w] += v.x, t[1][w] += v.y, t[2][w] += v.z, t[3][w] += v.w;
-              }
-              *to = make_float4(t[0][w], t[1][w], t[2][w], t[3][w]);
-            }
-      }
-      __syncthreads();
+      for (uint32_t w = 0; w < S::kTeams; ++w)
+        sum_l.add(make_float2(row_m[w][r * 16u + n], row_l[w][r * 16u + n]), top);
+      if (j == 0u) row_sum[r * 16u + n] = sum_l.result(top);
     }
+    const float mine = Joined::times(m[r], top);
+#pragma unroll
+    for (uint32_t u = 0; u < S::kPasses; ++u)
+#pragma unroll
+      for (uint32_t w = 0; w < 4; ++w)
+#pragma unroll
+        for (uint32_t d = 0; d < S::kEach; d += 4) {
+          const f32x4* t = &out[r][u * S::kEach + d];
+          *reinterpret_cast<float4*>(join + ((half * S::kPasses + u) * 16u + j * 4u + w) * S::kEach +
+                                     d) =
+              make_float4(t[0][w] * mine, t[1][w] * mine, t[2][w] * mine, t[3][w] * mine);
+        }
+    __syncthreads();
     constexpr uint32_t kRowThreads = kThreads / 16u;
     const uint32_t jr = tid / kRowThreads, jn = tid % kRowThreads, out_row = row0 + r * 16u + jr;
     if (out_row < rows) {
-      float2 st = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-      for (uint32_t w = 0; w < WAVES; ++w)
-        st = joined(st, make_float2(row_m[w][r * 16u + jr], row_l[w][r * 16u + jr]));
+      const float2 st = row_sum[r * 16u + jr];
       const size_t head = (size_t)kv * rows + out_row;
       const size_t part_row = (size_t)(share + seq) * c.kv_heads * rows + head;
-      const uint32_t t = out_row / a.group, h = kv * a.group + (out_row - t * a.group);
+      const uint32_t t = o.by_group.of(out_row), h = kv * a.group + (out_row - t * a.group);
       if (jn == 0u) {
-        if (shares != 1u) o.part_stats[part_row] = st;
+        if (!alone) o.part_stats[part_row] = st;
         else if (o.stats) o.stats[(size_t)seq * c.kv_heads * rows + head] = row_stats(st, T::kShift);
       }
-      float* to = shares == 1u ? a.out + (((size_t)seq * a.tokens + t) * a.heads + h) * dim
-                               : o.part_out + part_row * dim;
-      const float times = shares == 1u ? row_times(st) : 1.0f;
+      float* to = alone ? a.out + (((size_t)seq * a.tokens + t) * a.heads + h) * dim
+                        : o.part_out + part_row * dim;
+      const float times = alone ? row_times(st) : 1.0f;
       for (uint32_t d = jn * 4u; d < dim; d += 4u * kRowThreads) {
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (st.y != 0.0f) {  // (a row that sees nothing has no part in what its columns hold)
 #pragma unroll
-          for (uint32_t w = 0; w < WAVES / 2u; ++w) {
+          for (uint32_t w = 0; w < S::kTeams; ++w) {
             const float4 y = *reinterpret_cast<const float4*>(
                 reinterpret_cast<const float*>(shared) + (w * 16u + jr) * S::kOutStride + d);
             v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
@@ -596,56 +702,56 @@ __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void attention_mfma(Attention
       }
     }
   }
-  (void)last_share;
-  next_walk(a, kRound, walk);
+  next_sequence<kRound>(a, walk);
   if (walk.at < walk.end) __syncthreads();  // (the outputs are no longer read)
   }
 }
 
-template <typename T, uint32_t DC, bool FULL, uint32_t RT, uint32_t WAVES, uint32_t PER_SIMD>
+template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT>
 hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
-  using S = Shape<T, DC, RT, WAVES>;
+  using S = Shape<T, DW, VS, RT>;
   static const hipError_t attr = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(&attention_mfma<T, DC, FULL, RT, WAVES, PER_SIMD>),
+      reinterpret_cast<const void*>(&attention_mfma<T, DW, VS, FAST, RT>),
       hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::kShared);
   if (attr != hipSuccess) return attr;
   const uint32_t tiles = row_tiles(a.tokens, a.group);
   o.tile_groups = (tiles + RT - 1u) / RT;
-  o.round = T::kSlots * WAVES;
+  o.round = T::kSlots * S::kTeams;
   o.shift = T::kShift;
-  o.shares = shares_for(a.cache, o.tile_groups, PER_SIMD * 4u / WAVES, o.round);
+  o.shares = shares_for(a.cache, o.tile_groups, o.round);
+  o.by_shares = divisor_of(o.shares);
+  o.by_tiles = divisor_of(o.tile_groups);
   const uint32_t units = o.shares * a.cache.kv_heads;
   const uint32_t blocks = o.tile_groups == 1u ? units : (units + 7u) / 8u * 8u * o.tile_groups;
-  attention_mfma<T, DC, FULL, RT, WAVES, PER_SIMD><<<blocks, 64 * WAVES, S::kShared, s>>>(a, o);
+  attention_mfma<T, DW, VS, FAST, RT><<<blocks, 64 * S::kWaves, S::kShared, s>>>(a, o);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || o.shares == 1u) return e;
   return launch_attention_join(a, o, s);
 }
 
 // The row tiles a wave takes, so that the cache is read for several at once:
-// as many as leave registers for two waves a SIMD beside the tile; two of the
-// largest heads, as one wave of twice the registers.
-template <typename T, uint32_t DC, bool FULL>
+// as many as leave registers for two waves a SIMD beside the tile, three of an
+// f32 cache, two else.
+template <typename T, uint32_t DW, uint32_t VS>
 hipError_t launch_rows(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
   const uint32_t tiles = row_tiles(a.tokens, a.group);
-  if (tiles == 1u) return launch_mfma<T, DC, FULL, 1, 8, 2>(a, o, s);
-  if constexpr (DC == 256) return launch_mfma<T, DC, FULL, 1, 8, 2>(a, o, s);
-  if constexpr (DC == 64)
-    if (tiles == 3u || tiles > 4u) return launch_mfma<T, DC, FULL, 3, 8, 2>(a, o, s);
-  return launch_mfma<T, DC, FULL, 2, 8, 2>(a, o, s);
+  if (tiles == 1u) return launch_mfma<T, DW, VS, true, 1>(a, o, s);
+  if constexpr (T::kBytes == 4)
+    if (tiles == 3u || tiles > 4u) return launch_mfma<T, DW, VS, true, 3>(a, o, s);
+  return launch_mfma<T, DW, VS, true, 2>(a, o, s);
 }
 
 template <typename T>
 hipError_t launch_type(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
-  switch (a.cache.head_dim) {
-    case 64: return launch_rows<T, 64, true>(a, o, s);
-    case 128: return launch_rows<T, 128, true>(a, o, s);
-    case 256: return launch_rows<T, 256, true>(a, o, s);
-    default: break;
+  const uint32_t dim = a.cache.head_dim;
+  if (a.cache.page_tokens % 16u == 0u) {
+    if (dim == 64u) return launch_rows<T, 64, 1>(a, o, s);
+    if (dim == 128u) return launch_rows<T, 128, 1>(a, o, s);
+    if (dim == 256u) return launch_rows<T, 128, 2>(a, o, s);
   }
-  if (a.cache.head_dim < 64u) return launch_mfma<T, 64, false, 1, 8, 2>(a, o, s);
-  if (a.cache.head_dim < 128u) return launch_mfma<T, 128, false, 1, 8, 2>(a, o, s);
-  return launch_mfma<T, 256, false, 1, 8, 2>(a, o, s);
+  if (dim <= 64u) return launch_mfma<T, 64, 1, false, 1>(a, o, s);
+  if (dim <= 128u) return launch_mfma<T, 128, 1, false, 1>(a, o, s);
+  return launch_mfma<T, 128, 2, false, 1>(a, o, s);
 }
 
 }  // namespace attn

@@ -42,6 +42,16 @@ __host__ __device__ __forceinline__ uint32_t divided(uint32_t n, uint32_t mul, u
   return (uint32_t)(((uint64_t)n * mul) >> (31u + shift));
 }
 
+struct Divisor {
+  uint32_t mul, shift;
+  __host__ __device__ __forceinline__ uint32_t of(uint32_t n) const { return divided(n, mul, shift); }
+};
+inline Divisor divisor_of(uint32_t d) {
+  Divisor r;
+  division_by(d, &r.mul, &r.shift);
+  return r;
+}
+
 // The row of head `head` in slot `slot` of sequence `seq`; kNone where the
 // slot's page lies beyond the pool.  slot < capacity.
 __device__ __forceinline__ uint32_t cache_row(const CacheView& c, uint32_t seq, uint32_t head,

@@ -29,17 +29,22 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
     before += __shfl_xor(before, s, 64);
     total += __shfl_xor(total, s, 64);
   }
-  const uint32_t each = (total + o.shares - 1u) / o.shares;
+  const uint32_t each = o.by_shares.of(total + o.shares - 1u);
   const uint32_t share0 = before / each;
   const uint32_t shares =
       (before + span_of(a, seq, o.round).rounds - 1u) / each - share0 + 1u;
   if (shares == 1u) return;  // written already
   const auto at = [&](uint32_t p) { return (size_t)(share0 + p + seq) * c.kv_heads * rows + head; };
-  float2 st = make_float2(-INFINITY, 0.0f);
-  for (uint32_t p = lane; p < shares; p += 64u) st = joined(st, o.part_stats[at(p)]);
+  float top = -INFINITY;
+  for (uint32_t p = lane; p < shares; p += 64u) top = fmaxf(top, o.part_stats[at(p)].x);
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1)
-    st = joined(st, make_float2(__shfl_xor(st.x, s, 64), __shfl_xor(st.y, s, 64)));
+  for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+  Joined sum_l;
+  for (uint32_t p = lane; p < shares; p += 64u) sum_l.add(o.part_stats[at(p)], top);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum_l.l += __shfl_xor(sum_l.l, s, 64);
+  sum_l.minus = __builtin_amdgcn_ballot_w64(sum_l.minus) != 0u;
+  const float2 st = sum_l.result(top);
   const uint32_t dim = c.head_dim, width = dim / 4u, groups = kThreads / width;
   const uint32_t group = tid / width, d = (tid - group * width) * 4u;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -89,6 +94,8 @@ hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* 
   const uint32_t row = c.head_dim * (c.type == kKvF32 ? 4u : 2u);
   *taken =
       row % 16u == 0u && ((uintptr_t)c.keys | (uintptr_t)c.values | (uintptr_t)a.out) % 16u == 0u;
+  // (the rounds of all sequences are counted in 31 bits)
+  *taken = *taken && (uint64_t)c.sequences * (c.capacity / 64u + 2u) < 0x7fffffffu;
   if (!*taken) return hipSuccess;
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   Outputs o{};
@@ -97,6 +104,10 @@ hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* 
   o.stats = a.weights ? reinterpret_cast<float2*>(w + sp.stats) : nullptr;
   o.scores = a.weights ? reinterpret_cast<float*>(w + sp.scores) : nullptr;
   o.score_stride = sp.score_stride;
+  o.q_vectors = (uintptr_t)a.q % 16u == 0u && a.q_token_stride % 4u == 0u &&
+                a.q_head_stride % 4u == 0u;
+  o.by_group = divisor_of(a.group);
+  o.by_heads = divisor_of(c.kv_heads);
   if (c.type == kKvF32) return launch_attention_f32(a, o, s);
   if (c.type == kKvF16) return launch_attention_f16(a, o, s);
   return launch_attention_bf16(a, o, s);
