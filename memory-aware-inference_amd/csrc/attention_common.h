@@ -20,7 +20,7 @@ __host__ __device__ inline uint32_t row_tiles(uint32_t tokens, uint32_t group) {
 // the card's 8 XCDs of 32 CUs hold at once, one a CU, over the kv heads.  The
 // groups of row tiles of one share and head go to one XCD; one workgroup more
 // than an XCD has CUs would wait for a whole share (verified drafts of three
-// groups: 113 us for 33 workgroups on some XCDs, 62 us for 30).  No more than
+// groups: 113 us for 33 workgroups on some XCDs, 94 us for 30).  No more than
 // there can be rounds.
 constexpr uint32_t kXcds = 8, kXcdCus = 32;
 inline uint32_t shares_for(const CacheView& c, uint32_t tile_groups, uint32_t round) {
@@ -71,6 +71,7 @@ struct Outputs {
   float* part_out;     // and their outputs before the division
   float2* stats;       // with weights: (m, 1 / l) of every row, [sequences][kv_heads][rows]
   float* scores;
+  uint32_t* counters;  // of shares that are done, zeroed; null: a second kernel joins
   uint32_t score_stride, shares, tile_groups, round;
   float shift;  // p is held times 2^shift
   bool q_vectors;  // the queries can be read in sixteen-byte pieces
@@ -118,7 +119,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
 // once, a lane each.
 struct Walk {
   uint32_t lengths, counts, upto;  // the lane's sequence, and the rounds up to its last
-  uint32_t begin, limit, at, end;  // the rounds that are left: [at, end)
+  uint32_t each, begin, limit, at, end;  // the rounds that are left: [at, end)
   uint32_t seq, first;             // the present sequence, its first round
   Span span;
 };
@@ -167,10 +168,10 @@ __device__ __forceinline__ Walk first_walk(const AttentionArgs& a, const Outputs
     w.upto = total + wave_scan(rounds, lane);
     total = __builtin_amdgcn_readlane(w.upto, 63);
   }
-  const uint32_t each = o.by_shares.of(total + o.shares - 1u);
-  w.begin = w.at = min(share * each, total);
-  w.end = min(w.begin + each, total);
-  w.limit = w.begin + each;
+  w.each = o.by_shares.of(total + o.shares - 1u);
+  w.begin = w.at = min(share * w.each, total);
+  w.end = min(w.begin + w.each, total);
+  w.limit = w.begin + w.each;
   if (w.at >= w.end) return w;
   if (sequences <= 64u) {
     w.seq = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(w.at < w.upto));
@@ -229,6 +230,23 @@ __device__ __forceinline__ float2 row_stats(float2 st, float shift) {
   if (st.y == 0.0f) return make_float2(0.0f, 0.0f);
   return make_float2(st.x == -INFINITY ? 0.0f : st.x - shift, row_times(st));
 }
+
+// Four values of a share's output added at the share's weight, and what becomes
+// of the sum.
+__device__ __forceinline__ void add_share(float m, float top, const float4& x, float4& sum) {
+  const float w = m == -INFINITY ? 0.0f : exp2_of(m - top);
+  sum.x = fmaf(w, x.x, sum.x);
+  sum.y = fmaf(w, x.y, sum.y);
+  sum.z = fmaf(w, x.z, sum.z);
+  sum.w = fmaf(w, x.w, sum.w);
+}
+__device__ __forceinline__ float4 finished(float4 sum, float2 st) {
+  if (st.y == 0.0f) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const float t = row_times(st);
+  return make_float4(sum.x * t, sum.y * t, sum.z * t, sum.w * t);
+}
+
+constexpr uint32_t kSharesJoinedInside = 8;
 
 }  // namespace attn
 

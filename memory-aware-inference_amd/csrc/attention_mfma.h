@@ -153,7 +153,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
   extern __shared__ __attribute__((aligned(16))) uint8_t shared[];
   __shared__ float row_m[S::kTeams][RT * 16], row_l[S::kTeams][RT * 16];
   __shared__ float2 row_sum[RT * 16];
-  __shared__ uint32_t row_top[RT * 16];
+  __shared__ uint32_t row_top[RT * 16], last_share;
   const CacheView& c = a.cache;
   const uint32_t wave = uniform(threadIdx.x / 64u), team = wave / VS, half = wave % VS;
   const uint32_t dim = FAST ? DW * VS : c.head_dim;
@@ -702,6 +702,71 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       }
     }
   }
+  if (o.counters && !alone) {
+    // The last of the sequence's shares joins them.  Each wave waits for its
+    // stores; then one thread's release and acquire make this share's outputs
+    // known to the other XCDs, and theirs to this workgroup.
+    const uint32_t share0 = uniform(walk.first / walk.each);
+    const uint32_t shares = uniform((walk.first + walk.span.rounds - 1u) / walk.each) - share0 + 1u;
+    uint32_t* counter = o.counters + ((size_t)seq * c.kv_heads + kv) * o.tile_groups + group_at;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0u)
+      last_share = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+                   shares - 1u;
+    __syncthreads();
+    if (last_share) {
+      if (tid == 0u)
+        __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      constexpr uint32_t kRowThreads = kThreads / 16u;
+      for (uint32_t out_row = row0 + tid / kRowThreads; out_row < min(row0 + RT * 16u, rows);
+           out_row += 16u) {
+        const size_t head = (size_t)kv * rows + out_row;
+        const auto at = [&](uint32_t p) {
+          return (size_t)(share0 + p + seq) * c.kv_heads * rows + head;
+        };
+        // (all of it under way at once)
+        constexpr uint32_t kOuts = (DW * VS + 4u * kRowThreads - 1u) / (4u * kRowThreads);
+        float2 set[kSharesJoinedInside];
+        float4 x[kSharesJoinedInside][kOuts];
+#pragma unroll
+        for (uint32_t p = 0; p < kSharesJoinedInside; ++p) {
+          set[p] = make_float2(-INFINITY, 0.0f);
+          if (p < shares) set[p] = o.part_stats[at(p)];
+#pragma unroll
+          for (uint32_t k = 0; k < kOuts; ++k) {
+            const uint32_t d = (tid % kRowThreads + k * kRowThreads) * 4u;
+            x[p][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (p < shares && d < dim)
+              x[p][k] = *reinterpret_cast<const float4*>(o.part_out + at(p) * dim + d);
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t p = 0; p < kSharesJoinedInside; ++p) top = fmaxf(top, set[p].x);
+        Joined sum_l;
+        float4 v[kOuts];
+#pragma unroll
+        for (uint32_t k = 0; k < kOuts; ++k) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (uint32_t p = 0; p < kSharesJoinedInside; ++p) {
+          sum_l.add(set[p], top);
+#pragma unroll
+          for (uint32_t k = 0; k < kOuts; ++k) add_share(set[p].x, top, x[p][k], v[k]);
+        }
+        const float2 st = sum_l.result(top);
+        const uint32_t t = o.by_group.of(out_row), h = kv * a.group + (out_row - t * a.group);
+        float* to = a.out + (((size_t)seq * a.tokens + t) * a.heads + h) * dim;
+        if (o.stats && tid % kRowThreads == 0u)
+          o.stats[(size_t)seq * c.kv_heads * rows + head] = row_stats(st, T::kShift);
+#pragma unroll
+        for (uint32_t k = 0; k < kOuts; ++k) {
+          const uint32_t d = (tid % kRowThreads + k * kRowThreads) * 4u;
+          if (d < dim) *reinterpret_cast<float4*>(to + d) = finished(v[k], st);
+        }
+      }
+    }
+  }
   next_sequence<kRound>(a, walk);
   if (walk.at < walk.end) __syncthreads();  // (the outputs are no longer read)
   }
@@ -721,11 +786,17 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   o.shares = shares_for(a.cache, o.tile_groups, o.round);
   o.by_shares = divisor_of(o.shares);
   o.by_tiles = divisor_of(o.tile_groups);
+  // A few shares are joined by the last of them; many, whose join is more than
+  // one workgroup's work, by a kernel of their own.  (1021 slots of 8 heads
+  // of 128, four shares: 12.9 us inside, 14.8 with the second kernel.)
+  if (o.shares > kSharesJoinedInside ||
+      (size_t)a.cache.sequences * a.cache.kv_heads * o.tile_groups * 4u + 64u > kWorkspaceCounterBytes)
+    o.counters = nullptr;
   const uint32_t units = o.shares * a.cache.kv_heads;
   const uint32_t blocks = o.tile_groups == 1u ? units : (units + 7u) / 8u * 8u * o.tile_groups;
   attention_mfma<T, DW, VS, FAST, RT><<<blocks, 64 * S::kWaves, S::kShared, s>>>(a, o);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || o.shares == 1u) return e;
+  if (e != hipSuccess || o.shares == 1u || o.counters) return e;
   return launch_attention_join(a, o, s);
 }
 

@@ -51,14 +51,8 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
   if (group < groups) {
 #pragma unroll 4
     for (uint32_t p = group; p < shares; p += groups) {
-      const size_t row = at(p);
-      const float m = o.part_stats[row].x;
-      const float w = m == -INFINITY ? 0.0f : exp2_of(m - st.x);
-      const float4 x = *reinterpret_cast<const float4*>(o.part_out + row * dim + d);
-      sum.x = fmaf(w, x.x, sum.x);
-      sum.y = fmaf(w, x.y, sum.y);
-      sum.z = fmaf(w, x.z, sum.z);
-      sum.w = fmaf(w, x.w, sum.w);
+      add_share(o.part_stats[at(p)].x, top,
+                *reinterpret_cast<const float4*>(o.part_out + at(p) * dim + d), sum);
     }
     shared[group * width + d / 4u] = sum;
   }
@@ -68,14 +62,9 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
     const float4 x = shared[g * width + d / 4u];
     sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
   }
-  const float times = row_times(st);
   const uint32_t t = r / a.group, h = kv * a.group + (r - t * a.group);
   float* to = a.out + (((size_t)seq * a.tokens + t) * a.heads + h) * dim + d;
-  if (st.y != 0.0f)
-    sum = make_float4(sum.x * times, sum.y * times, sum.z * times, sum.w * times);
-  else
-    sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  *reinterpret_cast<float4*>(to) = sum;
+  *reinterpret_cast<float4*>(to) = finished(sum, st);
   if (o.stats && tid == 0u) o.stats[(size_t)seq * c.kv_heads * rows + head] = row_stats(st, o.shift);
 }
 
@@ -104,6 +93,7 @@ hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* 
   o.stats = a.weights ? reinterpret_cast<float2*>(w + sp.stats) : nullptr;
   o.scores = a.weights ? reinterpret_cast<float*>(w + sp.scores) : nullptr;
   o.score_stride = sp.score_stride;
+  o.counters = static_cast<uint32_t*>(a.report);
   o.q_vectors = (uintptr_t)a.q % 16u == 0u && a.q_token_stride % 4u == 0u &&
                 a.q_head_stride % 4u == 0u;
   o.by_group = divisor_of(a.group);
