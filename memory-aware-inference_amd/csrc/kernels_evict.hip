@@ -3,8 +3,12 @@
 // Weights are compared as 32-bit integers whose order is theirs, so the
 // selection is exact and its ties are too: the `need`-th largest integer T of
 // the slots between the first `sinks` and the last `recent` is found digit by
-// digit from histograms, then a pass over the slots in order keeps those above
-// T and the first ones equal to it.  A second kernel moves the kept rows.
+// digit from histograms in LDS, then the slots above T and the first ones
+// equal to it are kept.  A second kernel moves the kept rows; it is bound by
+// memory, the selection by the chain of its passes.  So a head's selection is
+// one workgroup's, whose threads read their slots, next to each other, once
+// and hold them (up to 32768 slots; more are read in each pass), and one scan
+// over the threads places all that is kept.
 #include "decode_internal.h"
 
 namespace sihip {
@@ -20,18 +24,19 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 // Exclusive sum of v over the workgroup's threads, and all of it.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* part, uint32_t& total) {
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* part, V& total) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
-  uint32_t x = v;
+  V x = v;
 #pragma unroll
   for (uint32_t o = 1; o < 64u; o <<= 1) {
-    const uint32_t y = __shfl_up(x, o, 64);
+    const V y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
   __syncthreads();
   if (lane == 63u) part[wave] = x;
   __syncthreads();
-  uint32_t before = 0u;
+  V before = 0u;
   total = 0u;
 #pragma unroll
   for (uint32_t i = 0; i < kWaves; ++i) {
@@ -42,16 +47,20 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* part, uint3
 }
 
 // grid (kv_heads, sequences): the kept slots of one head, and their weights.
-__global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
-  __shared__ uint32_t bins[2048], part[kWaves], found[2];
+// HELD: a thread's slots, in registers; 0: any number, read in each pass.
+template <uint32_t HELD>
+__global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a, bool vectors) {
+  __shared__ uint4 bins[2048];  // (four counts a bin, by lane, so that fewer wait for one)
+  __shared__ uint32_t part[kWaves], found[2], zeros;
+  __shared__ uint64_t part64[kWaves];
+  __shared__ uint16_t order[HELD ? HELD * kThreads : 1u];
   const CacheView& c = a.from;
   const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
   const size_t head = (size_t)s * c.kv_heads + h;
   const float* w = a.weights + head * a.weights_stride;
   float* to_w = a.to_weights + head * a.to_weights_stride;
   uint32_t* kept = a.kept + head * a.keep;
-  const uint32_t n = held(c, s);
-  const uint32_t left = min(n, a.keep);
+  const uint32_t n = held(c, s), left = min(n, a.keep);
   if (tid == 0u && h == 0u) {
     a.to.lengths[s] = left;
     if (c.lengths[s] > c.capacity) report_device_error(a.report, kDevErrCacheFull);
@@ -64,34 +73,103 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
     }
     return;
   }
-  // the need-th largest of the slots in [lo, hi)
+  // the thread's slots, in fours: [first, first + 4 fours)
+  const uint32_t fours = (n + 4u * kThreads - 1u) / (4u * kThreads), first = tid * 4u * fours;
+  const auto load = [&](uint32_t f) {
+    const uint32_t at = first + 4u * f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (vectors && at + 3u < n) {
+      v = *reinterpret_cast<const float4*>(w + at);
+    } else {
+      if (at < n) v.x = w[at];
+      if (at + 1u < n) v.y = w[at + 1u];
+      if (at + 2u < n) v.z = w[at + 2u];
+      if (at + 3u < n) v.w = w[at + 3u];
+    }
+    return v;
+  };
   const uint32_t lo = a.sinks, hi = n - a.recent;
+  // the held slots' ranks, and a bit for each: one of those in question; kept anyway
+  constexpr uint32_t kFours = HELD ? HELD / 4u : 1u;
+  uint32_t rank[4u * kFours], asked = 0u, safe = 0u;
+  if constexpr (HELD != 0u) {
+    float4 v[kFours];
+#pragma unroll
+    for (uint32_t f = 0; f < kFours; ++f) {
+      v[f] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (f < fours) v[f] = load(f);
+    }
+#pragma unroll
+    for (uint32_t f = 0; f < kFours; ++f) {
+      rank[4u * f] = rank_of(v[f].x), rank[4u * f + 1u] = rank_of(v[f].y);
+      rank[4u * f + 2u] = rank_of(v[f].z), rank[4u * f + 3u] = rank_of(v[f].w);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < HELD; ++j) {
+      const uint32_t i = first + j;
+      if (j < 4u * fours && i < n) (i >= lo && i < hi ? asked : safe) |= 1u << j;
+    }
+  }
+  // every slot in question with its rank
+  const auto each = [&](auto&& visit) {
+    if constexpr (HELD != 0u) {
+#pragma unroll
+      for (uint32_t j = 0; j < HELD; ++j)
+        if (asked >> j & 1u) visit(j, rank[j]);
+    } else {
+      for (uint32_t f = 0; f < fours; ++f) {
+        const float4 v = load(f);
+        const uint32_t i = first + 4u * f;
+        if (i >= lo && i < hi) visit(i, rank_of(v.x));
+        if (i + 1u >= lo && i + 1u < hi) visit(i + 1u, rank_of(v.y));
+        if (i + 2u >= lo && i + 2u < hi) visit(i + 2u, rank_of(v.z));
+        if (i + 3u >= lo && i + 3u < hi) visit(i + 3u, rank_of(v.w));
+      }
+    }
+  };
+  // the need-th largest of the slots in [lo, hi)
   uint32_t need = a.keep - a.sinks - a.recent, prefix = 0u, known = 0u;
+  const uint32_t zero = rank_of(0.0f);
   if (need != 0u) {
     for (uint32_t digit = 0; digit < 3u; ++digit) {
       const uint32_t shift = digit == 0u ? 21u : digit == 1u ? 10u : 0u;
       const uint32_t size = digit == 2u ? 1024u : 2048u;
-      for (uint32_t i = tid; i < size; i += kThreads) bins[i] = 0u;
+      for (uint32_t i = tid; i < size; i += kThreads) bins[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (tid == 0u) zeros = 0u;
       __syncthreads();
-      for (uint32_t i = lo + tid; i < hi; i += kThreads) {
-        const uint32_t k = rank_of(w[i]);
-        if ((k & known) == prefix) atomicAdd(&bins[(k >> shift) & (size - 1u)], 1u);
-      }
+      // (slots that nothing ever saw weigh 0, many of them: counted apart, they do not
+      // queue for one bin)
+      uint32_t nothing = 0u;
+      each([&](uint32_t, uint32_t k) {
+        if ((k & known) == prefix) {
+          if (k == zero) ++nothing;
+          else
+            atomicAdd(reinterpret_cast<uint32_t*>(bins) + 4u * ((k >> shift) & (size - 1u)) +
+                          (tid & 3u),
+                      1u);
+        }
+      });
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) nothing += __shfl_xor(nothing, o, 64);
+      if ((tid & 63u) == 0u && nothing != 0u) atomicAdd(&zeros, nothing);
       __syncthreads();
       // thread i has the bins size - 1 - (size / kThreads) i and below
-      const uint32_t each = size / kThreads;
-      uint32_t mine = 0u;
-      for (uint32_t j = 0; j < each; ++j) mine += bins[size - 1u - (tid * each + j)];
-      uint32_t total;
-      uint32_t before = block_scan(mine, part, total);
-      if (before < need && need <= before + mine)
-        for (uint32_t j = 0; j < each; ++j) {
-          const uint32_t bin = size - 1u - (tid * each + j);
-          if (before < need && need <= before + bins[bin]) {
-            found[0] = bin;
+      const uint32_t every = size / kThreads, zero_bin = (zero >> shift) & (size - 1u);
+      const auto bin_of = [&](uint32_t j) { return size - 1u - (tid * every + j); };
+      const auto count_of = [&](uint32_t b) {
+        return bins[b].x + bins[b].y + bins[b].z + bins[b].w + (b == zero_bin ? zeros : 0u);
+      };
+      uint32_t own = 0u, total;
+      for (uint32_t j = 0; j < every; ++j) own += count_of(bin_of(j));
+      uint32_t before = block_scan(own, part, total);
+      if (before < need && need <= before + own)
+        for (uint32_t j = 0; j < every; ++j) {
+          const uint32_t count = count_of(bin_of(j));
+          if (before < need && need <= before + count) {
+            found[0] = bin_of(j);
             found[1] = need - before;
           }
-          before += bins[bin];
+          before += count;
         }
       __syncthreads();
       prefix |= found[0] << shift;
@@ -100,24 +178,67 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
       __syncthreads();
     }
   }
-  // the slots above T and the first `need` equal to it (none where nothing is needed)
+  // what is kept: the slots outside, those above T, and the first `need` equal to it
   const bool none = known == 0u;
-  uint32_t out = 0u, ties = 0u;
-  for (uint32_t base = 0; base < n; base += kThreads) {
-    const uint32_t i = base + tid;
-    const bool inside = i >= lo && i < hi;
-    const uint32_t k = inside && !none ? rank_of(w[i]) : 0u;
-    const bool tie = inside && !none && k == prefix;
-    uint32_t total;
-    const uint32_t tie_rank = ties + block_scan(tie ? 1u : 0u, part, total);
-    ties += total;
-    const bool keep = i < n && (!inside || (!none && (k > prefix || (tie && tie_rank < need))));
-    const uint32_t at = out + block_scan(keep ? 1u : 0u, part, total);
-    out += total;
-    if (keep) {
-      kept[at] = i;
-      to_w[at] = w[i];
+  uint64_t total;
+  if constexpr (HELD != 0u) {
+    uint32_t equal = 0u;
+    if (!none)
+#pragma unroll
+      for (uint32_t j = 0; j < HELD; ++j) {
+        safe |= (asked >> j & 1u) != 0u && rank[j] > prefix ? 1u << j : 0u;
+        equal |= (asked >> j & 1u) != 0u && rank[j] == prefix ? 1u << j : 0u;
+      }
+    const uint64_t own = (uint64_t)__popc(safe) << 32 | __popc(equal);
+    const uint64_t before = block_scan(own, part64, total);
+    const uint32_t ties = (uint32_t)before;
+    for (uint32_t left_over = ties < need ? need - ties : 0u; equal != 0u && left_over != 0u;
+         --left_over) {
+      safe |= equal & -equal;
+      equal &= equal - 1u;
     }
+    // (a thread's slots go to places of their own: through LDS, so that the stores to
+    // memory are of whole lines)
+    for (uint32_t at = (uint32_t)(before >> 32) + min(ties, need); safe != 0u; safe &= safe - 1u)
+      order[at++] = (uint16_t)(first + (uint32_t)__ffs(safe) - 1u);
+    __syncthreads();
+    for (uint32_t i = tid; i < left; i += kThreads) {
+      const uint32_t slot = order[i];
+      kept[i] = slot;
+      to_w[i] = w[slot];
+    }
+  } else {
+    const auto kind = [&](uint32_t i, float v) -> uint32_t {  // 2: kept, 1: equal, 0: not
+      if (i >= n) return 0u;
+      if (i < lo || i >= hi) return 2u;
+      const uint32_t k = rank_of(v);
+      return none ? 0u : k > prefix ? 2u : k == prefix ? 1u : 0u;
+    };
+    const auto all = [&](auto&& visit) {
+      for (uint32_t f = 0; f < fours; ++f) {
+        const float4 v = load(f);
+        visit(first + 4u * f, v.x);
+        visit(first + 4u * f + 1u, v.y);
+        visit(first + 4u * f + 2u, v.z);
+        visit(first + 4u * f + 3u, v.w);
+      }
+    };
+    uint64_t own = 0u;
+    all([&](uint32_t i, float v) {
+      const uint32_t k = kind(i, v);
+      own += k == 2u ? 1ull << 32 : k;
+    });
+    const uint64_t before = block_scan(own, part64, total);
+    uint32_t ties = (uint32_t)before, at = (uint32_t)(before >> 32) + min(ties, need);
+    all([&](uint32_t i, float v) {
+      const uint32_t k = kind(i, v);
+      if (k == 2u || (k == 1u && ties < need)) {
+        kept[at] = i;
+        to_w[at] = v;
+        ++at;
+      }
+      ties += k & 1u;
+    });
   }
 }
 
@@ -151,7 +272,16 @@ __global__ __launch_bounds__(256) void evict_move(EvictArgs a, uint32_t units) {
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
   const CacheView& c = a.from;
-  evict_select<<<dim3(c.kv_heads, c.sequences), kThreads, 0, s>>>(a);
+  const dim3 heads(c.kv_heads, c.sequences);
+  const bool vectors = (uintptr_t)a.weights % 16u == 0u && a.weights_stride % 4u == 0u;
+  if (c.capacity <= 8u * kThreads)
+    evict_select<8><<<heads, kThreads, 0, s>>>(a, vectors);
+  else if (c.capacity <= 16u * kThreads)
+    evict_select<16><<<heads, kThreads, 0, s>>>(a, vectors);
+  else if (c.capacity <= 32u * kThreads)
+    evict_select<32><<<heads, kThreads, 0, s>>>(a, vectors);
+  else
+    evict_select<0><<<heads, kThreads, 0, s>>>(a, vectors);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t bytes = c.head_dim * (c.type == kKvF32 ? 4u : 2u);
