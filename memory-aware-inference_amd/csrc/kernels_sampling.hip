@@ -5,9 +5,29 @@ namespace sihip {
 namespace {
 
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
-constexpr uint32_t kEach = 16;                 // values a thread
-constexpr uint32_t kChunk = kThreads * kEach;  // values a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Values [base + 4 (j kThreads + thread), + 4), j < FOURS, of a row of `cols`;
+// `rest` where there is none.  VEC: rows that begin on sixteen bytes.
+template <bool VEC, uint32_t FOURS>
+__device__ __forceinline__ void load_fours(const float* row, size_t base, size_t cols, float rest,
+                                           float4 (&v)[FOURS]) {
+#pragma unroll
+  for (uint32_t j = 0; j < FOURS; ++j) {
+    const size_t c = base + 4u * (j * kThreads + threadIdx.x);
+    v[j] = make_float4(rest, rest, rest, rest);
+    if (VEC) {
+      if (c < cols) v[j] = *reinterpret_cast<const float4*>(row + c);
+    } else {
+      if (c < cols) v[j].x = row[c];
+      if (c + 1u < cols) v[j].y = row[c + 1u];
+      if (c + 2u < cols) v[j].z = row[c + 2u];
+      if (c + 3u < cols) v[j].w = row[c + 3u];
+    }
+  }
+}
 
 // ---- softmax ------------------------------------------------------------------
 // y = exp((x - m) / T) / l: a workgroup a chunk of a row, once for the chunk's
@@ -33,38 +53,51 @@ __device__ __forceinline__ float2 block_joined(float2 v, float per, float2* part
   return v;
 }
 
-// grid (chunks, rows)
+// grid (chunks, rows): a chunk is 4 FOURS values a thread
+template <bool VEC, uint32_t FOURS>
 __global__ __launch_bounds__(kThreads) void softmax_stats(const float* __restrict__ x, size_t cols,
                                                           float per, float2* stats) {
   __shared__ float2 part[kWaves];
-  const float* row = x + blockIdx.y * cols;
-  const size_t base = (size_t)blockIdx.x * kChunk;
-  float v[kEach], m = -INFINITY, sum = 0.0f;
+  float4 v[FOURS];
+  load_fours<VEC>(x + blockIdx.y * cols, (size_t)blockIdx.x * 4u * FOURS * kThreads, cols,
+                  -INFINITY, v);
+  float m = -INFINITY, sum = 0.0f;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; ++i) {
-    const size_t c = base + i * kThreads + threadIdx.x;
-    v[i] = c < cols ? row[c] : -INFINITY;
-    m = fmaxf(m, v[i]);
-  }
+  for (uint32_t j = 0; j < FOURS; ++j) m = fmaxf(fmaxf(fmaxf(m, v[j].x), fmaxf(v[j].y, v[j].z)), v[j].w);
   const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; ++i) sum += exp2f((v[i] - from) * per);
+  for (uint32_t j = 0; j < FOURS; ++j)
+    sum += (exp2f((v[j].x - from) * per) + exp2f((v[j].y - from) * per)) +
+           (exp2f((v[j].z - from) * per) + exp2f((v[j].w - from) * per));
   const float2 r = block_joined(make_float2(m, sum), per, part);
   if (threadIdx.x == 0u) stats[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = r;
 }
+template <bool VEC, uint32_t FOURS>
 __global__ __launch_bounds__(kThreads) void softmax_values(const float* x, size_t cols, float per,
                                                            const float2* stats, float* y) {
   __shared__ float2 part[kWaves];
+  const size_t base = (size_t)blockIdx.x * 4u * FOURS * kThreads;
+  float4 v[FOURS];
+  load_fours<VEC>(x + blockIdx.y * cols, base, cols, 0.0f, v);
   const float2* st = stats + (size_t)blockIdx.y * gridDim.x;
   float2 r = make_float2(-INFINITY, 0.0f);
   for (uint32_t i = threadIdx.x; i < gridDim.x; i += kThreads) r = joined(r, st[i], per);
   r = block_joined(r, per, part);
   const float from = r.x == -INFINITY ? 0.0f : r.x, scale = 1.0f / r.y;
-  const size_t row = blockIdx.y * cols, base = (size_t)blockIdx.x * kChunk;
+  float* row = y + blockIdx.y * cols;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; ++i) {
-    const size_t c = base + i * kThreads + threadIdx.x;
-    if (c < cols) y[row + c] = exp2f((x[row + c] - from) * per) * scale;
+  for (uint32_t j = 0; j < FOURS; ++j) {
+    const size_t c = base + 4u * (j * kThreads + threadIdx.x);
+    const f32x4 e{exp2f((v[j].x - from) * per) * scale, exp2f((v[j].y - from) * per) * scale,
+                  exp2f((v[j].z - from) * per) * scale, exp2f((v[j].w - from) * per) * scale};
+    if (VEC) {
+      if (c < cols) __builtin_nontemporal_store(e, reinterpret_cast<f32x4*>(row + c));
+    } else {
+      if (c < cols) row[c] = e.x;
+      if (c + 1u < cols) row[c + 1u] = e.y;
+      if (c + 2u < cols) row[c + 2u] = e.z;
+      if (c + 3u < cols) row[c + 3u] = e.w;
+    }
   }
 }
 
@@ -72,25 +105,59 @@ __global__ __launch_bounds__(kThreads) void softmax_values(const float* x, size_
 // Terms in 2^-36 fixed point: their sums are exact in any order, so the
 // workgroups' shares of a row add up to what one pass over it would give.
 
-// floor(clamp(x, 0, 1) 2^36); a NaN is 0.  The 24-bit significand, moved.
+// floor(clamp(x, 0, 1) 2^36) = high 2^18 + low; a NaN is 0.  x 2^18 less its
+// whole part has no more bits than x, so both conversions are exact.  Sums of
+// up to 2^13 terms stay within 32 bits in each half.
+struct Fixed {
+  uint32_t high = 0u, low = 0u;
+  __device__ __forceinline__ void add(float x) {
+    const float y = fminf(fmaxf(x, 0.0f), 1.0f) * 0x1p18f;
+    const uint32_t h = (uint32_t)y;
+    high += h;
+    low += (uint32_t)((y - (float)h) * 0x1p18f);
+  }
+  __device__ __forceinline__ uint64_t value() const { return ((uint64_t)high << 18) + low; }
+};
 __device__ __forceinline__ uint64_t fixed(float x) {
-  if (!(x > 0.0f)) return 0u;
-  const uint32_t b = __float_as_uint(fminf(x, 1.0f));
-  const uint32_t e = b >> 23;  // x = (b & mask | 2^23) 2^(e - 150)
-  const uint64_t m = (b & 0x7fffffu) | 0x800000u;
-  return e >= 114u ? m << (e - 114u) : e > 90u ? m >> (114u - e) : 0u;
+  Fixed f;
+  f.add(x);
+  return f.value();
 }
 
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* part) {
+// A workgroup's sum of its threads' terms, for thread 0.
+__device__ __forceinline__ uint64_t block_sum(Fixed v, uint64_t* part) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = 32; o > 0; o >>= 1) {
+    v.high += __shfl_xor(v.high, o, 64);
+    v.low += __shfl_xor(v.low, o, 64);
+  }
+  if ((threadIdx.x & 63u) == 0u) part[threadIdx.x / 64u] = v.value();
   __syncthreads();
-  if ((threadIdx.x & 63u) == 0u) part[threadIdx.x / 64u] = v;
-  __syncthreads();
-  v = 0u;
+  uint64_t total = 0u;
 #pragma unroll
-  for (uint32_t i = 0; i < kWaves; ++i) v += part[i];
-  return v;
+  for (uint32_t i = 0; i < kWaves; ++i) total += part[i];
+  return total;
+}
+
+// Sum of v over the workgroup's threads up to and with this one, and of all.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t& total) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
+#pragma unroll
+  for (uint32_t o = 1; o < 64u; o <<= 1) {
+    const uint64_t y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 63u) part[wave] = v;
+  __syncthreads();
+  uint64_t before = 0u;
+  total = 0u;
+#pragma unroll
+  for (uint32_t i = 0; i < kWaves; ++i) {
+    if (i < wave) before += part[i];
+    total += part[i];
+  }
+  return before + v;
 }
 
 // Where a sequence's drafts end: how many are accepted, of how many.
@@ -137,96 +204,137 @@ __device__ __forceinline__ Rows rows_of(const VerifyArgs& a, uint32_t s, const E
   }
   return r;
 }
-__device__ __forceinline__ uint64_t rest_of(const Rows& r, uint32_t v, float p) {
-  if (r.q) return fixed(p - r.q[v]);
-  return fixed(v == r.certain ? p - 1.0f : p);
+// Device-coherent (sc1) accesses: each XCD has its own L2.
+__device__ __forceinline__ void store_coherent(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t load_coherent(const uint64_t* p) {
+  return __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// grid (chunks, sequences): the chunk's sums of max(p - q, 0) and of p
-__global__ __launch_bounds__(kThreads) void verify_sums(VerifyArgs a, ulonglong2* sums) {
-  __shared__ uint32_t shared[3];
-  __shared__ uint64_t part[kWaves];
-  const uint32_t s = blockIdx.y, base = blockIdx.x * kChunk;
-  const Ends e = ends_of(a, s, shared);
-  const Rows r = rows_of(a, s, e);
-  uint64_t rest = 0u, all = 0u;
+// The values of a row that a workgroup takes: 16 a thread, next to each other.
+constexpr uint32_t kEach = 16, kChunk = kThreads * kEach;
+
+template <bool VEC>
+__device__ __forceinline__ void load_each(const float* row, uint32_t first, uint32_t vocab,
+                                          float (&v)[kEach]) {
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; ++i) {
-    const uint32_t v = base + i * kThreads + threadIdx.x;
-    if (v < a.vocab) {
-      const float p = r.p[v];
-      rest += rest_of(r, v, p);
-      all += fixed(p);
+  for (uint32_t i = 0; i < kEach; i += 4) {
+    if (VEC) {
+      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (first + i < vocab) f = *reinterpret_cast<const float4*>(row + first + i);
+      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) v[i + k] = first + i + k < vocab ? row[first + i + k] : 0.0f;
     }
   }
-  rest = block_sum(rest, part);
-  all = block_sum(all, part);
-  if (threadIdx.x == 0u)
-    sums[(size_t)s * gridDim.x + blockIdx.x] = make_ulonglong2(rest, all);
 }
 
-// grid (sequences): the token whose running sum first exceeds the threshold
-__global__ __launch_bounds__(kThreads) void verify_draw(VerifyArgs a, const ulonglong2* sums,
-                                                        uint32_t chunks, void* ws) {
-  __shared__ uint32_t shared[3], at;
+// grid (chunks, sequences): each workgroup adds up its chunk's max(p - q, 0); the
+// one that is done last finds the token whose running sum first exceeds the
+// threshold: its chunk from the chunks' sums, then its place in that chunk.
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, uint64_t* sums,
+                                                          uint32_t* counters, void* ws) {
+  __shared__ uint32_t shared[3], is_last, at;
   __shared__ uint64_t part[kWaves], left;
-  const uint32_t s = blockIdx.x, tid = threadIdx.x;
+  const uint32_t s = blockIdx.y, tid = threadIdx.x, chunks = gridDim.x;
   const Ends e = ends_of(a, s, shared);
   Rows r = rows_of(a, s, e);
   sums += (size_t)s * chunks;
-  uint64_t rest = 0u, all = 0u;
-  for (uint32_t i = tid; i < chunks; i += kThreads) {
-    rest += sums[i].x;
-    all += sums[i].y;
+  // the thread's values of a chunk, p or what is left of it
+  float v[kEach];
+  const auto load = [&](uint32_t chunk) {
+    const uint32_t first = chunk * kChunk + tid * kEach;
+    load_each<VEC>(r.p, first, a.vocab, v);
+    if (r.q) {
+      float q[kEach];
+      load_each<VEC>(r.q, first, a.vocab, q);
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) v[i] -= q[i];
+    } else if (r.certain - first < kEach) {
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i)
+        if (first + i == r.certain) v[i] -= 1.0f;
+    }
+  };
+  const auto own = [&] {
+    Fixed f;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) f.add(v[i]);
+    return f;
+  };
+  load(blockIdx.x);
+  const uint64_t sum = block_sum(own(), part);
+  if (tid == 0u) {
+    // Device-coherent stores, in place before the chunk is counted, and read by loads of
+    // the same kind: the sums are known to the last workgroup on whatever XCD without a
+    // write-back of its L2.
+    store_coherent(sums + blockIdx.x, sum);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    is_last = __hip_atomic_fetch_add(counters + s, 1u, __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT) == chunks - 1u;
+    if (is_last)
+      __hip_atomic_store(counters + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  rest = block_sum(rest, part);
-  all = block_sum(all, part);
-  const bool whole = rest == 0u;  // p itself (the same sums where nothing was taken away)
-  if (whole) r.q = nullptr, r.certain = kNone;
-  const uint64_t total = whole ? all : rest;
+  __syncthreads();
+  if (!is_last) return;
+  // the chunks' sums: a thread's are next to each other
+  const uint32_t per = (chunks + kThreads - 1u) / kThreads;
+  const uint32_t c0 = min(tid * per, chunks), c1 = min(c0 + per, chunks);
+  uint64_t mine, upto, total;
+  const auto add_chunks = [&] {
+    mine = 0u;
+    for (uint32_t i = c0; i < c1; ++i) mine += load_coherent(sums + i);
+    upto = block_scan(mine, part, total);
+  };
+  add_chunks();
+  if (total == 0u && (r.q || r.certain != kNone)) {
+    // nothing is left of p: p itself (rare, so its sums are taken here)
+    r.q = nullptr;
+    r.certain = kNone;
+    for (uint32_t c = 0; c < chunks; ++c) {
+      load(c);
+      __syncthreads();
+      const uint64_t one = block_sum(own(), part);
+      if (tid == 0u) store_coherent(sums + c, one);
+    }
+    if (tid == 0u) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    add_chunks();
+  }
   const float u = a.uniform[(size_t)s * (a.drafts + 1u) + a.drafts];
   const uint32_t n24 = u > 0.0f ? (uint32_t)fminf(u * 0x1p24f, 16777215.0f) : 0u;
-  const uint64_t lo = total * n24, hi = __umul64hi(total, n24);
-  const uint64_t threshold = hi << 40 | lo >> 24;
-  // the chunk: sums up to it, one after another
-  if (tid == 0u) {
-    uint64_t before = 0u;
-    uint32_t c = 0u;
-    if (total != 0u)
-      for (;; ++c) {
-        const uint64_t one = whole ? sums[c].y : sums[c].x;
-        if (before + one > threshold) break;
-        before += one;
-      }
-    at = c;
+  const uint64_t threshold = __umul64hi(total, n24) << 40 | (total * n24) >> 24;
+  if (total != 0u && upto - mine <= threshold && threshold < upto) {
+    uint64_t before = upto - mine;
+    uint32_t i = c0;
+    for (;; ++i) {
+      const uint64_t one = load_coherent(sums + i);
+      if (before + one > threshold) break;
+      before += one;
+    }
+    at = i;
     left = threshold - before;
   }
   __syncthreads();
-  // its values: a thread's are next to each other
-  const uint32_t first = at * kChunk + tid * kEach;
-  uint64_t mine = 0u;
-  for (uint32_t i = 0; i < kEach; ++i)
-    if (first + i < a.vocab) mine += rest_of(r, first + i, r.p[first + i]);
-  uint64_t upto = mine;
-  const uint32_t lane = tid & 63u, wave = tid / 64u;
-#pragma unroll
-  for (uint32_t o = 1; o < 64u; o <<= 1) {
-    const uint64_t y = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += y;
-  }
-  __syncthreads();
-  if (lane == 63u) part[wave] = upto;
-  __syncthreads();
-  for (uint32_t i = 0; i < wave; ++i) upto += part[i];
   uint32_t* out = a.out_tokens + (size_t)s * (a.drafts + 1u);
-  if (total != 0u && upto > left && upto - mine <= left) {
-    uint64_t before = upto - mine;
-    uint32_t v = first;
-    for (;; ++v) {
-      before += rest_of(r, v, r.p[v]);
-      if (before > left) break;
+  if (total != 0u) {
+    load(at);
+    uint64_t whole;
+    mine = own().value();
+    upto = block_scan(mine, part, whole);
+    if (upto - mine <= left && left < upto) {
+      uint64_t running = upto - mine;
+      uint32_t token = kNone;
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) {
+        running += fixed(v[i]);
+        if (token == kNone && running > left) token = at * kChunk + tid * kEach + i;
+      }
+      out[e.accepted] = token;
     }
-    out[e.accepted] = v;
   }
   if (tid == 0u) {
     a.accepted[s] = e.accepted;
@@ -240,28 +348,49 @@ __global__ __launch_bounds__(kThreads) void verify_draw(VerifyArgs a, const ulon
     out[tid] = tid < e.accepted ? a.tokens[(size_t)s * a.drafts + tid] : kNone;
 }
 
-}  // namespace
-
-hipError_t launch_softmax(const float* x, float* y, size_t rows, size_t cols, float temperature,
-                          const Workspace& ws, hipStream_t s) {
-  const uint32_t chunks = (uint32_t)((cols + kChunk - 1u) / kChunk);
+template <bool VEC, uint32_t FOURS>
+hipError_t softmax_rows(const float* x, float* y, size_t rows, size_t cols, float per,
+                        const Workspace& ws, hipStream_t s) {
+  const uint32_t chunk = 4u * FOURS * kThreads, chunks = (uint32_t)((cols + chunk - 1u) / chunk);
   const size_t most = std::min<size_t>(ws.scratch_bytes / sizeof(float2) / chunks, 65535u);
-  const float per = kLog2e / temperature;
   float2* stats = reinterpret_cast<float2*>(ws.scratch);
   for (size_t r = 0; r < rows; r += most) {
     const dim3 grid(chunks, (uint32_t)std::min(most, rows - r));
-    softmax_stats<<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats);
-    softmax_values<<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats, y + r * cols);
+    softmax_stats<VEC, FOURS><<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats);
+    softmax_values<VEC, FOURS><<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats,
+                                                         y + r * cols);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0u; }
+
+}  // namespace
+
+hipError_t launch_softmax(const float* x, float* y, size_t rows, size_t cols, float temperature,
+                          const Workspace& ws, hipStream_t s) {
+  const float per = kLog2e / temperature;
+  const bool vec = cols % 4u == 0u && aligned16(x) && aligned16(y);
+  // Chunks of 8192 values where there are workgroups enough for the card, else of 2048, so
+  // that a few rows have more of them.
+  const bool many = rows * ((cols + 8191u) / 8192u) >= 1024u;
+  if (vec)
+    return many ? softmax_rows<true, 8>(x, y, rows, cols, per, ws, s)
+                : softmax_rows<true, 2>(x, y, rows, cols, per, ws, s);
+  return many ? softmax_rows<false, 8>(x, y, rows, cols, per, ws, s)
+              : softmax_rows<false, 2>(x, y, rows, cols, per, ws, s);
+}
+
 hipError_t launch_verify(const VerifyArgs& a, const Workspace& ws, hipStream_t s) {
   const uint32_t chunks = (a.vocab + kChunk - 1u) / kChunk;
-  ulonglong2* sums = reinterpret_cast<ulonglong2*>(ws.scratch);
-  const uint32_t most = (uint32_t)std::min<size_t>(ws.scratch_bytes / sizeof(ulonglong2) / chunks, 65535u);
+  uint64_t* sums = reinterpret_cast<uint64_t*>(ws.scratch);
+  uint32_t* counters = static_cast<uint32_t*>(ws.ptr);  // at rest zero, and left so
+  static_assert(65535u * 4u + 64u <= kWorkspaceCounterBytes, "a counter for each sequence");
+  const uint32_t most =
+      (uint32_t)std::min<size_t>(ws.scratch_bytes / sizeof(uint64_t) / chunks, 65535u);
+  const bool vec = a.vocab % 4u == 0u && aligned16(a.target) && aligned16(a.draft);
   for (uint32_t n = 0; n < a.sequences; n += most) {
     VerifyArgs b = a;
     b.sequences = std::min(most, a.sequences - n);
@@ -272,8 +401,11 @@ hipError_t launch_verify(const VerifyArgs& a, const Workspace& ws, hipStream_t s
     b.uniform += (size_t)n * (a.drafts + 1u);
     b.accepted += n;
     b.out_tokens += (size_t)n * (a.drafts + 1u);
-    verify_sums<<<dim3(chunks, b.sequences), kThreads, 0, s>>>(b, sums);
-    verify_draw<<<b.sequences, kThreads, 0, s>>>(b, sums, chunks, ws.ptr);
+    const dim3 grid(chunks, b.sequences);
+    if (vec)
+      verify_kernel<true><<<grid, kThreads, 0, s>>>(b, sums, counters, ws.ptr);
+    else
+      verify_kernel<false><<<grid, kThreads, 0, s>>>(b, sums, counters, ws.ptr);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
