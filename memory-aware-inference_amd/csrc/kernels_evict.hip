@@ -242,31 +242,55 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a, bool vecto
   }
 }
 
-// grid (rows / rows a workgroup, kv_heads, sequences): U is the unit that rows
-// are moved in.
+// grid (rows, kv_heads, sequences): U is the unit that rows are moved in.  A
+// thread has four rows under way at once, each behind three dependent reads
+// (its slot, the page, the row).  The rows are not used again here: their
+// stores pass the caches by.
+constexpr uint32_t kMoveThreads = 256, kMoveRows = 4;
 template <typename U>
-__global__ __launch_bounds__(256) void evict_move(EvictArgs a, uint32_t units) {
+__global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs a, uint32_t units) {
   const uint32_t h = blockIdx.y, s = blockIdx.z;
   const uint32_t left = min(held(a.from, s), a.keep);
   const uint32_t* kept = a.kept + ((size_t)s * a.from.kv_heads + h) * a.keep;
-  const uint32_t rows = 256u / units ? 256u / units : 1u;
-  const uint32_t mine = threadIdx.x / units, u0 = threadIdx.x - mine * units;
-  if (mine >= rows) return;
-  for (uint32_t i = blockIdx.x * rows + mine; i < left; i += gridDim.x * rows) {
-    const uint32_t src = cache_row(a.from, s, h, kept[i]);
-    const uint32_t dst = cache_row(a.to, s, h, i);
-    if (src == kNone || dst == kNone) {
-      if (u0 == 0u) report_device_error(a.report, kDevErrCachePage);
-      continue;
+  const uint32_t rows = kMoveThreads / units;  // (a row has at most as many units)
+  const uint32_t row = threadIdx.x / units, u = threadIdx.x - row * units;
+  if (row >= rows) return;
+  const U* keys = static_cast<const U*>(a.from.keys);
+  const U* values = static_cast<const U*>(a.from.values);
+  for (uint32_t i0 = blockIdx.x * rows * kMoveRows + row; i0 < left;
+       i0 += gridDim.x * rows * kMoveRows) {
+    uint32_t src[kMoveRows], dst[kMoveRows];
+#pragma unroll
+    for (uint32_t k = 0; k < kMoveRows; ++k) {
+      const uint32_t i = i0 + k * rows;
+      src[k] = i < left ? kept[i] : 0u;
     }
-    for (uint32_t u = u0; u < units; u += 256u) {
-      static_cast<U*>(a.to.keys)[(size_t)dst * units + u] =
-          static_cast<const U*>(a.from.keys)[(size_t)src * units + u];
-      static_cast<U*>(a.to.values)[(size_t)dst * units + u] =
-          static_cast<const U*>(a.from.values)[(size_t)src * units + u];
+    U key[kMoveRows], value[kMoveRows];
+#pragma unroll
+    for (uint32_t k = 0; k < kMoveRows; ++k) {
+      const uint32_t i = i0 + k * rows;
+      src[k] = i < left ? cache_row(a.from, s, h, src[k]) : kNone;
+      dst[k] = i < left ? cache_row(a.to, s, h, i) : kNone;
+      if (i < left && (src[k] == kNone || dst[k] == kNone) && u == 0u)
+        report_device_error(a.report, kDevErrCachePage);
     }
+#pragma unroll
+    for (uint32_t k = 0; k < kMoveRows; ++k)
+      if (src[k] != kNone && dst[k] != kNone) {
+        key[k] = keys[(size_t)src[k] * units + u];
+        value[k] = values[(size_t)src[k] * units + u];
+      }
+#pragma unroll
+    for (uint32_t k = 0; k < kMoveRows; ++k)
+      if (src[k] != kNone && dst[k] != kNone) {
+        __builtin_nontemporal_store(key[k], static_cast<U*>(a.to.keys) + (size_t)dst[k] * units + u);
+        __builtin_nontemporal_store(value[k],
+                                    static_cast<U*>(a.to.values) + (size_t)dst[k] * units + u);
+      }
   }
 }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 }  // namespace
 
@@ -288,12 +312,12 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
   uintptr_t at = (uintptr_t)c.keys | (uintptr_t)c.values | (uintptr_t)a.to.keys |
                  (uintptr_t)a.to.values | bytes;
   auto go = [&](auto kernel, uint32_t units) {
-    const uint32_t rows = std::max(1u, 256u / units);
+    const uint32_t rows = kMoveThreads / units * kMoveRows;
     const uint32_t blocks = std::min((a.keep + rows - 1u) / rows, 65535u);
-    kernel<<<dim3(blocks, c.kv_heads, c.sequences), 256, 0, s>>>(a, units);
+    kernel<<<dim3(blocks, c.kv_heads, c.sequences), kMoveThreads, 0, s>>>(a, units);
   };
   if (at % 16u == 0u)
-    go(evict_move<uint4>, bytes / 16u);
+    go(evict_move<u32x4>, bytes / 16u);
   else if (at % 4u == 0u)
     go(evict_move<uint32_t>, bytes / 4u);
   else
