@@ -331,7 +331,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
   uint32_t largest = 0u;
   if (!S::kInRegisters && T::kShift != 0.0f) {
     if (tid < RT * 16u) row_top[tid] = 0u;
-    __syncthreads();
+    exchange_barrier();
   }
 #pragma unroll
   for (uint32_t k = 0; k < kMine; ++k) {
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       largest = max(largest, (uint32_t)__shfl_xor(largest, 16, 64));
       largest = max(largest, (uint32_t)__shfl_xor(largest, 32, 64));
     } else {
-      __syncthreads();
+      exchange_barrier();
     }
   }
   // the row's power of two, 2^14 at the largest value; 1 where that is no number
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       else q_lds[q * S::kItems + i] = w[q];
     }
   }
-  if (!S::kInRegisters) __syncthreads();
+  if (!S::kInRegisters) exchange_barrier();
   load_values(row);
 
   // ---- the lane's rows, and their slots
@@ -649,7 +649,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
   float* join = reinterpret_cast<float*>(shared) + (team * 16u + n) * S::kOutStride;
 #pragma unroll
   for (uint32_t r = 0; r < RT; ++r) {
-    __syncthreads();  // (the queries and scores, or the last tile's outputs, are no longer read)
+    exchange_barrier();  // (the queries and scores, or the last tile's outputs, are no longer read)
     float top = -INFINITY;
 #pragma unroll
     for (uint32_t w = 0; w < S::kTeams; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
                                      d) =
               make_float4(t[0][w] * mine, t[1][w] * mine, t[2][w] * mine, t[3][w] * mine);
         }
-    __syncthreads();
+    exchange_barrier();
     constexpr uint32_t kRowThreads = kThreads / 16u;
     const uint32_t jr = tid / kRowThreads, jn = tid % kRowThreads, out_row = row0 + r * 16u + jr;
     if (out_row < rows) {
@@ -710,11 +710,11 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     const uint32_t shares = uniform((walk.first + walk.span.rounds - 1u) / walk.each) - share0 + 1u;
     uint32_t* counter = o.counters + ((size_t)seq * c.kv_heads + kv) * o.tile_groups + group_at;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    exchange_barrier();
     if (tid == 0u)
       last_share = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
                    shares - 1u;
-    __syncthreads();
+    exchange_barrier();
     if (last_share) {
       if (tid == 0u)
         __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -768,7 +768,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     }
   }
   next_sequence<kRound>(a, walk);
-  if (walk.at < walk.end) __syncthreads();  // (the outputs are no longer read)
+  if (walk.at < walk.end) exchange_barrier();  // (the outputs are no longer read)
   }
 }
 

@@ -29,10 +29,9 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
     before += __shfl_xor(before, s, 64);
     total += __shfl_xor(total, s, 64);
   }
-  const uint32_t each = o.by_shares.of(total + o.shares - 1u);
-  const uint32_t share0 = before / each;
-  const uint32_t shares =
-      (before + span_of(a, seq, o.round).rounds - 1u) / each - share0 + 1u;
+  const Deal deal = deal_of(total, c.sequences, o);
+  const uint32_t first = before + deal.start * seq, share0 = first / deal.each;
+  const uint32_t shares = (first + span_of(a, seq, o.round).rounds - 1u) / deal.each - share0 + 1u;
   if (shares == 1u) return;  // written already
   const auto at = [&](uint32_t p) { return (size_t)(share0 + p + seq) * c.kv_heads * rows + head; };
   float top = -INFINITY;
@@ -84,7 +83,7 @@ hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* 
   *taken =
       row % 16u == 0u && ((uintptr_t)c.keys | (uintptr_t)c.values | (uintptr_t)a.out) % 16u == 0u;
   // (the rounds of all sequences are counted in 31 bits)
-  *taken = *taken && (uint64_t)c.sequences * (c.capacity / 64u + 2u) < 0x7fffffffu;
+  *taken = *taken && (uint64_t)c.sequences * (c.capacity / 64u + 3u) < 0x7fffffffu;
   if (!*taken) return hipSuccess;
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   Outputs o{};
