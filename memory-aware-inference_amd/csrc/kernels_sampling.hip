@@ -7,25 +7,36 @@ namespace {
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+// Four values at once: the card's sixteen-byte accesses need four-byte alignment, so rows
+// of an odd number of values take them too (288 rows of 151,936 logits, moved by four bytes:
+// 134 us value by value, 83 so; 81 where they begin on sixteen bytes).
+typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Whether a row ends inside four values of the chunk of `fours` a thread from `base` on.
+__device__ __forceinline__ bool ends_inside(size_t base, size_t cols, uint32_t fours) {
+  return cols % 4u != 0u && base + 4u * fours * kThreads > cols;
+}
 
 // Values [base + 4 (j kThreads + thread), + 4), j < FOURS, of a row of `cols`;
-// `rest` where there is none.  VEC: rows that begin on sixteen bytes.
-template <bool VEC, uint32_t FOURS>
+// `rest` where there is none.
+template <uint32_t FOURS>
 __device__ __forceinline__ void load_fours(const float* row, size_t base, size_t cols, float rest,
                                            float4 (&v)[FOURS]) {
 #pragma unroll
   for (uint32_t j = 0; j < FOURS; ++j) {
     const size_t c = base + 4u * (j * kThreads + threadIdx.x);
-    v[j] = make_float4(rest, rest, rest, rest);
-    if (VEC) {
-      if (c < cols) v[j] = *reinterpret_cast<const float4*>(row + c);
-    } else {
-      if (c < cols) v[j].x = row[c];
-      if (c + 1u < cols) v[j].y = row[c + 1u];
-      if (c + 2u < cols) v[j].z = row[c + 2u];
-      if (c + 3u < cols) v[j].w = row[c + 3u];
-    }
+    f32x4 f{rest, rest, rest, rest};
+    if (c + 3u < cols) f = *reinterpret_cast<const f32x4*>(row + c);
+    v[j] = make_float4(f.x, f.y, f.z, f.w);
+  }
+  if (!ends_inside(base, cols, FOURS)) return;
+#pragma unroll
+  for (uint32_t j = 0; j < FOURS; ++j) {
+    const size_t c = base + 4u * (j * kThreads + threadIdx.x);
+    if (c + 3u < cols) continue;
+    if (c < cols) v[j].x = row[c];
+    if (c + 1u < cols) v[j].y = row[c + 1u];
+    if (c + 2u < cols) v[j].z = row[c + 2u];
   }
 }
 
@@ -54,12 +65,12 @@ __device__ __forceinline__ float2 block_joined(float2 v, float per, float2* part
 }
 
 // grid (chunks, rows): a chunk is 4 FOURS values a thread
-template <bool VEC, uint32_t FOURS>
+template <uint32_t FOURS>
 __global__ __launch_bounds__(kThreads) void softmax_stats(const float* __restrict__ x, size_t cols,
                                                           float per, float2* stats) {
   __shared__ float2 part[kWaves];
   float4 v[FOURS];
-  load_fours<VEC>(x + blockIdx.y * cols, (size_t)blockIdx.x * 4u * FOURS * kThreads, cols,
+  load_fours(x + blockIdx.y * cols, (size_t)blockIdx.x * 4u * FOURS * kThreads, cols,
                   -INFINITY, v);
   float m = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -72,32 +83,35 @@ __global__ __launch_bounds__(kThreads) void softmax_stats(const float* __restric
   const float2 r = block_joined(make_float2(m, sum), per, part);
   if (threadIdx.x == 0u) stats[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = r;
 }
-template <bool VEC, uint32_t FOURS>
+template <uint32_t FOURS>
 __global__ __launch_bounds__(kThreads) void softmax_values(const float* x, size_t cols, float per,
                                                            const float2* stats, float* y) {
   __shared__ float2 part[kWaves];
   const size_t base = (size_t)blockIdx.x * 4u * FOURS * kThreads;
   float4 v[FOURS];
-  load_fours<VEC>(x + blockIdx.y * cols, base, cols, 0.0f, v);
+  load_fours(x + blockIdx.y * cols, base, cols, 0.0f, v);
   const float2* st = stats + (size_t)blockIdx.y * gridDim.x;
   float2 r = make_float2(-INFINITY, 0.0f);
   for (uint32_t i = threadIdx.x; i < gridDim.x; i += kThreads) r = joined(r, st[i], per);
   r = block_joined(r, per, part);
   const float from = r.x == -INFINITY ? 0.0f : r.x, scale = 1.0f / r.y;
   float* row = y + blockIdx.y * cols;
+  f32x4 e[FOURS];
 #pragma unroll
   for (uint32_t j = 0; j < FOURS; ++j) {
     const size_t c = base + 4u * (j * kThreads + threadIdx.x);
-    const f32x4 e{exp2f((v[j].x - from) * per) * scale, exp2f((v[j].y - from) * per) * scale,
-                  exp2f((v[j].z - from) * per) * scale, exp2f((v[j].w - from) * per) * scale};
-    if (VEC) {
-      if (c < cols) __builtin_nontemporal_store(e, reinterpret_cast<f32x4*>(row + c));
-    } else {
-      if (c < cols) row[c] = e.x;
-      if (c + 1u < cols) row[c + 1u] = e.y;
-      if (c + 2u < cols) row[c + 2u] = e.z;
-      if (c + 3u < cols) row[c + 3u] = e.w;
-    }
+    e[j] = f32x4{exp2f((v[j].x - from) * per) * scale, exp2f((v[j].y - from) * per) * scale,
+                 exp2f((v[j].z - from) * per) * scale, exp2f((v[j].w - from) * per) * scale};
+    if (c + 3u < cols) __builtin_nontemporal_store(e[j], reinterpret_cast<f32x4*>(row + c));
+  }
+  if (!ends_inside(base, cols, FOURS)) return;
+#pragma unroll
+  for (uint32_t j = 0; j < FOURS; ++j) {
+    const size_t c = base + 4u * (j * kThreads + threadIdx.x);
+    if (c + 3u < cols) continue;
+    if (c < cols) row[c] = e[j].x;
+    if (c + 1u < cols) row[c + 1u] = e[j].y;
+    if (c + 2u < cols) row[c + 2u] = e[j].z;
   }
 }
 
@@ -215,14 +229,12 @@ __device__ __forceinline__ uint64_t load_coherent(const uint64_t* p) {
 // The values of a row that a workgroup takes: 16 a thread, next to each other.
 constexpr uint32_t kEach = 16, kChunk = kThreads * kEach;
 
-template <bool VEC>
 __device__ __forceinline__ void load_each(const float* row, uint32_t first, uint32_t vocab,
                                           float (&v)[kEach]) {
 #pragma unroll
   for (uint32_t i = 0; i < kEach; i += 4) {
-    if (VEC) {
-      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (first + i < vocab) f = *reinterpret_cast<const float4*>(row + first + i);
+    if (first + i + 3u < vocab) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(row + first + i);
       v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
     } else {
 #pragma unroll
@@ -234,7 +246,6 @@ __device__ __forceinline__ void load_each(const float* row, uint32_t first, uint
 // grid (chunks, sequences): each workgroup adds up its chunk's max(p - q, 0); the
 // one that is done last finds the token whose running sum first exceeds the
 // threshold: its chunk from the chunks' sums, then its place in that chunk.
-template <bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, uint64_t* sums,
                                                           uint32_t* counters, void* ws) {
   __shared__ uint32_t shared[3], is_last, at;
@@ -247,10 +258,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, uint64_t
   float v[kEach];
   const auto load = [&](uint32_t chunk) {
     const uint32_t first = chunk * kChunk + tid * kEach;
-    load_each<VEC>(r.p, first, a.vocab, v);
+    load_each(r.p, first, a.vocab, v);
     if (r.q) {
       float q[kEach];
-      load_each<VEC>(r.q, first, a.vocab, q);
+      load_each(r.q, first, a.vocab, q);
 #pragma unroll
       for (uint32_t i = 0; i < kEach; ++i) v[i] -= q[i];
     } else if (r.certain - first < kEach) {
@@ -348,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, uint64_t
     out[tid] = tid < e.accepted ? a.tokens[(size_t)s * a.drafts + tid] : kNone;
 }
 
-template <bool VEC, uint32_t FOURS>
+template <uint32_t FOURS>
 hipError_t softmax_rows(const float* x, float* y, size_t rows, size_t cols, float per,
                         const Workspace& ws, hipStream_t s) {
   const uint32_t chunk = 4u * FOURS * kThreads, chunks = (uint32_t)((cols + chunk - 1u) / chunk);
@@ -356,8 +367,8 @@ hipError_t softmax_rows(const float* x, float* y, size_t rows, size_t cols, floa
   float2* stats = reinterpret_cast<float2*>(ws.scratch);
   for (size_t r = 0; r < rows; r += most) {
     const dim3 grid(chunks, (uint32_t)std::min(most, rows - r));
-    softmax_stats<VEC, FOURS><<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats);
-    softmax_values<VEC, FOURS><<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats,
+    softmax_stats<FOURS><<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats);
+    softmax_values<FOURS><<<grid, kThreads, 0, s>>>(x + r * cols, cols, per, stats,
                                                          y + r * cols);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -365,22 +376,17 @@ hipError_t softmax_rows(const float* x, float* y, size_t rows, size_t cols, floa
   return hipSuccess;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0u; }
-
 }  // namespace
 
 hipError_t launch_softmax(const float* x, float* y, size_t rows, size_t cols, float temperature,
                           const Workspace& ws, hipStream_t s) {
   const float per = kLog2e / temperature;
-  const bool vec = cols % 4u == 0u && aligned16(x) && aligned16(y);
-  // Chunks of 8192 values where there are workgroups enough for the card, else of 2048, so
-  // that a few rows have more of them.
-  const bool many = rows * ((cols + 8191u) / 8192u) >= 1024u;
-  if (vec)
-    return many ? softmax_rows<true, 8>(x, y, rows, cols, per, ws, s)
-                : softmax_rows<true, 2>(x, y, rows, cols, per, ws, s);
-  return many ? softmax_rows<false, 8>(x, y, rows, cols, per, ws, s)
-              : softmax_rows<false, 2>(x, y, rows, cols, per, ws, s);
+  // Chunks of 8192 values where they make a workgroup a CU, else of 2048, so that a few rows
+  // have more of them (of 151,936 logits 24 rows 10.1 us by 8192 and 12.0 by 2048, 16 rows
+  // 9.8 both; 5 rows 7.0 by 2048).
+  const bool many = rows * ((cols + 8191u) / 8192u) >= 256u;
+  return many ? softmax_rows<8>(x, y, rows, cols, per, ws, s)
+              : softmax_rows<2>(x, y, rows, cols, per, ws, s);
 }
 
 hipError_t launch_verify(const VerifyArgs& a, const Workspace& ws, hipStream_t s) {
@@ -390,7 +396,6 @@ hipError_t launch_verify(const VerifyArgs& a, const Workspace& ws, hipStream_t s
   static_assert(65535u * 4u + 64u <= kWorkspaceCounterBytes, "a counter for each sequence");
   const uint32_t most =
       (uint32_t)std::min<size_t>(ws.scratch_bytes / sizeof(uint64_t) / chunks, 65535u);
-  const bool vec = a.vocab % 4u == 0u && aligned16(a.target) && aligned16(a.draft);
   for (uint32_t n = 0; n < a.sequences; n += most) {
     VerifyArgs b = a;
     b.sequences = std::min(most, a.sequences - n);
@@ -402,10 +407,7 @@ hipError_t launch_verify(const VerifyArgs& a, const Workspace& ws, hipStream_t s
     b.accepted += n;
     b.out_tokens += (size_t)n * (a.drafts + 1u);
     const dim3 grid(chunks, b.sequences);
-    if (vec)
-      verify_kernel<true><<<grid, kThreads, 0, s>>>(b, sums, counters, ws.ptr);
-    else
-      verify_kernel<false><<<grid, kThreads, 0, s>>>(b, sums, counters, ws.ptr);
+    verify_kernel<<<grid, kThreads, 0, s>>>(b, sums, counters, ws.ptr);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

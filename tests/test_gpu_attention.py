@@ -249,6 +249,20 @@ def test_many_sequences(hip_ctx, dev):
     run(hip_ctx, dev, c, rng.standard_normal((333, 1, 4, 64)).astype(np.float32), weights=True)
 
 
+@pytest.mark.parametrize("sequences", [2, 3, 17, 63, 64, 65, 130])
+@pytest.mark.parametrize("kind,heads,dim,tokens", [("f16", 2, 64, 1), ("bf16", 3, 256, 7), ("f32", 2, 128, 9)])
+def test_shares_end_anywhere(hip_ctx, dev, kind, heads, dim, tokens, sequences):
+    """Batches of lengths from none to many rounds: shares that begin and end
+    inside sequences, between them, and over several of them."""
+    rng = np.random.default_rng(sequences)
+    lengths = np.where(rng.random(sequences) < 0.3, rng.integers(800, 3500, sequences),
+                       rng.integers(0, 300, sequences))
+    c = R.Cache(dev, rng, kind, sequences, 1, dim, 16, 3520 // 16, lengths)
+    counts = rng.integers(0, tokens + 1, sequences).astype(np.uint32)
+    q = rng.standard_normal((sequences, tokens, heads, dim)).astype(np.float32)
+    run(hip_ctx, dev, c, q, weights=sequences in (3, 65), counts=counts)
+
+
 def test_cache_beyond_four_gigabytes(hip_ctx, dev):
     """Pages at both ends of a pool of more than 2^32 values."""
     kv, dim, page = 1, 128, 64
