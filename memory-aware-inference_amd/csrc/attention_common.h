@@ -74,7 +74,6 @@ struct Outputs {
   uint32_t* counters;  // of shares that are done, zeroed; null: a second kernel joins
   uint32_t score_stride, shares, tile_groups, round;
   float shift;  // p is held times 2^shift
-  bool q_vectors;  // the queries can be read in sixteen-byte pieces
   Divisor by_group, by_heads, by_shares, by_tiles;  // group, kv_heads, shares, tile_groups
 };
 

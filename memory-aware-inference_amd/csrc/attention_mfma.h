@@ -266,7 +266,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       for (uint32_t k = 0; k < S::kSteps; ++k) {
         uint32_t at = ((half * S::kSteps + k) * 4u + j) * 16u;
         if (!FAST) at = min(at, row_bytes - 16u);  // (its query values are 0)
-        key[s][k] = *reinterpret_cast<const u32x4*>(p + at);
+        key[s][k] = *reinterpret_cast<const Words4*>(p + at);
       }
     }
   };
@@ -280,11 +280,11 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
         uint32_t at = ((half * S::kPasses + u) * 16u + n) * (S::kWords * 4u);
         if (!FAST) at = min(at, row_bytes - S::kWords * 4u);  // (its outputs are not stored)
         if constexpr (S::kWords == 4) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(p + at);
+          const u32x4 w = *reinterpret_cast<const Words4*>(p + at);
 #pragma unroll
           for (uint32_t x = 0; x < 4; ++x) value[i][u][x] = w[x];
         } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(p + at);
+          const Words2 w = *reinterpret_cast<const Words2*>(p + at);
           value[i][u][0] = w.x;
           value[i][u][1] = w.y;
         }
@@ -311,16 +311,11 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     const bool there = i < S::kItems && r < rows && t < count && d0 < dim;
     const float* src = a.q + ((size_t)seq * a.tokens + t) * a.q_token_stride +
                        (kv * a.group + (r - t * a.group)) * a.q_head_stride + d0;
-    if (o.q_vectors) {
 #pragma unroll
-      for (uint32_t v = 0; v < S::kValues; v += 4) {
-        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (there) f = *reinterpret_cast<const float4*>(src + v);
-        x[k][v] = f.x, x[k][v + 1] = f.y, x[k][v + 2] = f.z, x[k][v + 3] = f.w;
-      }
-    } else {
-#pragma unroll
-      for (uint32_t v = 0; v < S::kValues; ++v) x[k][v] = there ? src[v] : 0.0f;
+    for (uint32_t v = 0; v < S::kValues; v += 4) {
+      Floats4 f{0.0f, 0.0f, 0.0f, 0.0f};
+      if (there) f = *reinterpret_cast<const Floats4*>(src + v);
+      x[k][v] = f.x, x[k][v + 1] = f.y, x[k][v + 2] = f.z, x[k][v + 3] = f.w;
     }
   }
   Place row = rows_of(first, page);
@@ -698,7 +693,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
           }
           v.x *= times, v.y *= times, v.z *= times, v.w *= times;
         }
-        *reinterpret_cast<float4*>(to + d) = v;
+        *reinterpret_cast<Floats4*>(to + d) = Floats4{v.x, v.y, v.z, v.w};
       }
     }
   }
@@ -762,7 +757,8 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
         for (uint32_t k = 0; k < kOuts; ++k) {
           const uint32_t d = (tid % kRowThreads + k * kRowThreads) * 4u;
-          if (d < dim) *reinterpret_cast<float4*>(to + d) = finished(v[k], st);
+          const float4 f = finished(v[k], st);
+          if (d < dim) *reinterpret_cast<Floats4*>(to + d) = Floats4{f.x, f.y, f.z, f.w};
         }
       }
     }

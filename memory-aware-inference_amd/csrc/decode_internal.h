@@ -16,6 +16,13 @@ enum KvType : uint32_t { kKvF32 = 0, kKvF16 = 1, kKvBF16 = 30 };  // ggml type i
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr uint32_t kMaxHeadDim = 256;  // SI_HIP_MAX_HEAD_DIM
 
+// Sixteen and eight bytes of memory that is aligned to four: the card's wide
+// accesses need no more.
+typedef float Floats4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t Words2 __attribute__((ext_vector_type(2), aligned(4)));
+inline bool aligned4(const void* p) { return ((uintptr_t)p & 3u) == 0u; }
+
 // A si_hip_kv_cache as the kernels take it.  Rows (one head's values of one
 // slot) are numbered through the pool: (page * kv_heads + head) * page_tokens +
 // the slot's place in its page; the host has checked that the numbers fit

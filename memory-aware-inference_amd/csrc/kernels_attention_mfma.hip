@@ -63,7 +63,8 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
   }
   const uint32_t t = r / a.group, h = kv * a.group + (r - t * a.group);
   float* to = a.out + (((size_t)seq * a.tokens + t) * a.heads + h) * dim + d;
-  *reinterpret_cast<float4*>(to) = finished(sum, st);
+  const float4 v = finished(sum, st);
+  *reinterpret_cast<Floats4*>(to) = Floats4{v.x, v.y, v.z, v.w};
   if (o.stats && tid == 0u) o.stats[(size_t)seq * c.kv_heads * rows + head] = row_stats(st, o.shift);
 }
 
@@ -78,10 +79,9 @@ hipError_t launch_attention_join(const AttentionArgs& a, const Outputs& o, hipSt
 hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* taken,
                                  hipStream_t s) {
   const CacheView& c = a.cache;
-  // sixteen-byte loads of keys and values, and stores of the output
+  // rows of whole sixteen-byte pieces, whose words are words of memory
   const uint32_t row = c.head_dim * (c.type == kKvF32 ? 4u : 2u);
-  *taken =
-      row % 16u == 0u && ((uintptr_t)c.keys | (uintptr_t)c.values | (uintptr_t)a.out) % 16u == 0u;
+  *taken = row % 16u == 0u && aligned4(c.keys) && aligned4(c.values);
   // (the rounds of all sequences are counted in 31 bits)
   *taken = *taken && (uint64_t)c.sequences * (c.capacity / 64u + 3u) < 0x7fffffffu;
   if (!*taken) return hipSuccess;
@@ -93,8 +93,6 @@ hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* 
   o.scores = a.weights ? reinterpret_cast<float*>(w + sp.scores) : nullptr;
   o.score_stride = sp.score_stride;
   o.counters = static_cast<uint32_t*>(a.report);
-  o.q_vectors = (uintptr_t)a.q % 16u == 0u && a.q_token_stride % 4u == 0u &&
-                a.q_head_stride % 4u == 0u;
   o.by_group = divisor_of(a.group);
   o.by_heads = divisor_of(c.kv_heads);
   if (c.type == kKvF32) return launch_attention_f32(a, o, s);

@@ -290,8 +290,6 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs a, uint32_t
   }
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 }  // namespace
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
@@ -309,16 +307,16 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t bytes = c.head_dim * (c.type == kKvF32 ? 4u : 2u);
-  uintptr_t at = (uintptr_t)c.keys | (uintptr_t)c.values | (uintptr_t)a.to.keys |
-                 (uintptr_t)a.to.values | bytes;
+  const bool words =
+      aligned4(c.keys) && aligned4(c.values) && aligned4(a.to.keys) && aligned4(a.to.values);
   auto go = [&](auto kernel, uint32_t units) {
     const uint32_t rows = kMoveThreads / units * kMoveRows;
     const uint32_t blocks = std::min((a.keep + rows - 1u) / rows, 65535u);
     kernel<<<dim3(blocks, c.kv_heads, c.sequences), kMoveThreads, 0, s>>>(a, units);
   };
-  if (at % 16u == 0u)
-    go(evict_move<u32x4>, bytes / 16u);
-  else if (at % 4u == 0u)
+  if (words && bytes % 16u == 0u)
+    go(evict_move<Words4>, bytes / 16u);
+  else if (words && bytes % 4u == 0u)
     go(evict_move<uint32_t>, bytes / 4u);
   else
     go(evict_move<uint16_t>, bytes / 2u);

@@ -36,12 +36,12 @@ struct Row {
 template <uint32_t N, typename T>
 __device__ __forceinline__ void store_units(T* y, const float* v) {
   if constexpr (N == 4 && sizeof(T) == 2) {
-    union { T t[4]; uint2 u; } w;
+    union { T t[4]; Words2 u; } w;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) w.t[i] = to_type<T>(v[i]);
-    *reinterpret_cast<uint2*>(y) = w.u;
+    *reinterpret_cast<Words2*>(y) = w.u;
   } else if constexpr (N == 4) {
-    *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<Floats4*>(y) = Floats4{v[0], v[1], v[2], v[3]};
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) y[i] = to_type<T>(v[i]);
@@ -50,7 +50,7 @@ __device__ __forceinline__ void store_units(T* y, const float* v) {
 template <uint32_t N>
 __device__ __forceinline__ void load_units(float* v, const float* x) {
   if constexpr (N == 4) {
-    const float4 f = *reinterpret_cast<const float4*>(x);
+    const Floats4 f = *reinterpret_cast<const Floats4*>(x);
     v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
   } else {
 #pragma unroll
@@ -60,7 +60,8 @@ __device__ __forceinline__ void load_units(float* v, const float* x) {
 
 // Units of a row that a thread takes one of.  N = 4: sixteen-byte accesses,
 // four pairs of the half layout or two of the interleaved; N = 1: one pair, or
-// one value behind the rotated ones, at any alignment.  A pair is one thread's,
+// one value behind the rotated ones, for sizes that are no whole units and
+// 16-bit pools on odd halves of a word.  A pair is one thread's,
 // so a row may be rotated in place.
 __device__ __forceinline__ uint32_t row_units(uint32_t n, uint32_t dim, uint32_t layout, uint32_t N) {
   const uint32_t rotated = N == 4 && layout == 1u ? n / 4u : n / (2u * N);
@@ -193,8 +194,6 @@ __global__ void kv_advance_kernel(CacheView cache, const uint32_t* __restrict__ 
   cache.lengths[s] = (uint32_t)(n < cache.capacity ? n : cache.capacity);
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0u; }
-
 // Whether sixteen-byte units cover a row: its rotated part is whole units of
 // them (half layout: each half), and so is the rest.
 bool rope_vectors(uint32_t n, uint32_t dim, uint32_t layout) {
@@ -212,10 +211,7 @@ uint32_t slices_for(uint32_t tokens, uint32_t heads) {
 
 hipError_t launch_rope(const RopeArgs& rope, const RopeRows& rows, uint32_t tokens,
                        uint32_t head_dim, const uint32_t* positions, hipStream_t s) {
-  const bool vec = rope_vectors(rope.rotary_dim, head_dim, rope.layout) && aligned16(rows.x) &&
-                   aligned16(rows.y) && rows.token_stride % 4u == 0u &&
-                   rows.head_stride % 4u == 0u && rows.y_token_stride % 4u == 0u &&
-                   rows.y_head_stride % 4u == 0u;
+  const bool vec = rope_vectors(rope.rotary_dim, head_dim, rope.layout);
   const dim3 grid(tokens, slices_for(tokens, rows.heads));
   if (vec)
     rope_kernel<4><<<grid, kThreads, 0, s>>>(rope, rows, head_dim, positions);
@@ -230,11 +226,8 @@ hipError_t launch_rope_append(const CacheView& cache, const RopeArgs* rope, uint
                               void* ws, hipStream_t s) {
   const RopeArgs r = rope ? *rope : RopeArgs{0u, 0u, 1.0f, nullptr};
   const RopeRows qr = q ? *q : RopeRows{};
-  const bool vec = rope_vectors(r.rotary_dim, cache.head_dim, r.layout) && aligned16(k) &&
-                   aligned16(v) && aligned16(cache.keys) && aligned16(cache.values) &&
-                   k_stride % 4u == 0u && v_stride % 4u == 0u &&
-                   (!q || (aligned16(q->x) && aligned16(q->y) && q->token_stride % 4u == 0u &&
-                           q->head_stride % 4u == 0u));
+  const bool vec = rope_vectors(r.rotary_dim, cache.head_dim, r.layout) && aligned4(cache.keys) &&
+                   aligned4(cache.values);
   const uint32_t rows = cache.sequences * tokens;
   const dim3 grid(rows, slices_for(rows, qr.heads + 2u * cache.kv_heads));
   auto go = [&](auto kernel) {

@@ -7,10 +7,9 @@ namespace {
 constexpr uint32_t kThreads = 256, kWaves = kThreads / 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Four values at once: the card's sixteen-byte accesses need four-byte alignment, so rows
-// of an odd number of values take them too (288 rows of 151,936 logits, moved by four bytes:
-// 134 us value by value, 83 so; 81 where they begin on sixteen bytes).
-typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+// Rows of an odd number of values are read and written four values at once too (288 rows of
+// 151,936 logits, moved by four bytes: 134 us value by value, 83 so; 81 where they begin on
+// sixteen bytes).
 
 // Whether a row ends inside four values of the chunk of `fours` a thread from `base` on.
 __device__ __forceinline__ bool ends_inside(size_t base, size_t cols, uint32_t fours) {
@@ -25,8 +24,8 @@ __device__ __forceinline__ void load_fours(const float* row, size_t base, size_t
 #pragma unroll
   for (uint32_t j = 0; j < FOURS; ++j) {
     const size_t c = base + 4u * (j * kThreads + threadIdx.x);
-    f32x4 f{rest, rest, rest, rest};
-    if (c + 3u < cols) f = *reinterpret_cast<const f32x4*>(row + c);
+    Floats4 f{rest, rest, rest, rest};
+    if (c + 3u < cols) f = *reinterpret_cast<const Floats4*>(row + c);
     v[j] = make_float4(f.x, f.y, f.z, f.w);
   }
   if (!ends_inside(base, cols, FOURS)) return;
@@ -96,13 +95,13 @@ __global__ __launch_bounds__(kThreads) void softmax_values(const float* x, size_
   r = block_joined(r, per, part);
   const float from = r.x == -INFINITY ? 0.0f : r.x, scale = 1.0f / r.y;
   float* row = y + blockIdx.y * cols;
-  f32x4 e[FOURS];
+  Floats4 e[FOURS];
 #pragma unroll
   for (uint32_t j = 0; j < FOURS; ++j) {
     const size_t c = base + 4u * (j * kThreads + threadIdx.x);
-    e[j] = f32x4{exp2f((v[j].x - from) * per) * scale, exp2f((v[j].y - from) * per) * scale,
+    e[j] = Floats4{exp2f((v[j].x - from) * per) * scale, exp2f((v[j].y - from) * per) * scale,
                  exp2f((v[j].z - from) * per) * scale, exp2f((v[j].w - from) * per) * scale};
-    if (c + 3u < cols) __builtin_nontemporal_store(e[j], reinterpret_cast<f32x4*>(row + c));
+    if (c + 3u < cols) __builtin_nontemporal_store(e[j], reinterpret_cast<Floats4*>(row + c));
   }
   if (!ends_inside(base, cols, FOURS)) return;
 #pragma unroll
@@ -234,7 +233,7 @@ __device__ __forceinline__ void load_each(const float* row, uint32_t first, uint
 #pragma unroll
   for (uint32_t i = 0; i < kEach; i += 4) {
     if (first + i + 3u < vocab) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(row + first + i);
+      const Floats4 f = *reinterpret_cast<const Floats4*>(row + first + i);
       v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
     } else {
 #pragma unroll
