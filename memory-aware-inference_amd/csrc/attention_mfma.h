@@ -21,16 +21,29 @@
 // half loses bits to F16's range.  An f32 cache takes the f32 instructions.
 // Products and sums are f32.
 //
-// A wave has up to 128 values of a head.  Of a larger one two waves take a half
-// each, of the keys and of the values: they add their halves' scores through
-// LDS, and both go on with the sums.  The queries of one row tile stay in
-// registers; those of several are in LDS.
+// A wave has up to 128 values of a head.  Larger heads are a team's.  For one
+// row tile two waves take a half each, of the keys and of the values: they add
+// their halves' scores through LDS, and both go on with the sums.  For several
+// (kBySlots) the p of a row would be worked out by every wave of the team: so
+// four waves take a sixteen of slots each, with whole keys, agree on the rows'
+// maxima, put their p, in pieces, into LDS, and take a quarter of the values of
+// all their slots.  The queries of one row tile stay in registers; those of
+// several are in LDS.
 //
-// The slots of all sequences, in rounds of one tile for each team of waves of a
-// workgroup, are dealt to the workgroups of a kv head in equal shares, one
-// after another: a share may end one sequence and begin others.  A sequence
-// inside one share is written at once; the sums of one that lies in several
-// are joined in the order of the shares.
+// The slots of all sequences, in rounds of the tiles of a workgroup's teams,
+// are dealt to the workgroups of a kv head in equal shares, one after another:
+// a share may end one sequence and begin others.  A sequence inside one share is
+// written at once; the sums of one that lies in several are joined in the order
+// of the shares.
+//
+// Measured, calls back to back over caches that are not in the L2: one token
+// over 131,071 slots of 4 heads of 256 in BF16 104 us for 537 MB, 5.2 TB/s
+// (5.6 in this kernel), bound by memory; one token a sequence of 24 in F32,
+// 427 MB, 105 us with the weights, of which this kernel has 89; eight drafted
+// tokens a sequence of four, 183 MB, 61 us, bound by the arithmetic of a round
+// and by what comes before the first and behind the last (7 and 4 us); one
+// token over 1021 slots of 8 heads of 128, 4.2 MB, 12.4 us: the launch and a
+// chain of dependent reads (lengths, page numbers, rows, other shares' sums).
 #pragma once
 
 #include "attention_common.h"
@@ -113,14 +126,23 @@ struct Shape {
   static constexpr uint32_t kWords = kEach * T::kBytes / 4;
   static constexpr uint32_t kTiles = DW / 16;  // of the wave's output
   static constexpr bool kInRegisters = RT == 1;  // the queries
+  // how a team shares the scores: a sixteen of its slots a wave, or a part of the head
+  static constexpr bool kBySlots = VS == 4;
+  static constexpr uint32_t kOwnSubs = kBySlots ? 1 : kSubs;  // score tiles of a wave
+  static constexpr uint32_t kOwnRows = 4 * kOwnSubs;          // and a lane's slots in them
+  static constexpr uint32_t kKeySteps = kBySlots ? VS * kSteps : kSteps;
+  static constexpr uint32_t kTeamTiles = kBySlots ? VS / kSubs : 1;
+  static constexpr uint32_t kTeamSlots = kTeamTiles * T::kSlots, kRound = kTeams * kTeamSlots;
+  static constexpr uint32_t kSets = kBySlots ? kWaves : kTeams;  // of maxima and sums
   static constexpr uint32_t kItems = VS * RT * kSteps * 64;  // 16-byte pieces of the queries
   static constexpr uint32_t kQueryBytes = kInRegisters ? 0 : T::kPieces * kItems * 16;
-  // halves of scores that the waves of a team exchange
-  static constexpr uint32_t kBuffers = VS == 1 ? 0 : RT > 2 ? 1 : 2;
-  static constexpr uint32_t kExchange = kWaves * RT * kSubs * 64 * 16;
+  // what the waves of a team exchange: p, or halves of scores
+  static constexpr uint32_t kHalves = kWaves * kSubs * 64 * 16;
+  static constexpr uint32_t kExchangeBytes =
+      VS == 1 ? 0 : kBySlots ? kTeams * kTeamTiles * RT * T::kPieces * 64 * 16 : 2 * kHalves;
   static constexpr uint32_t kOutStride = DW * VS + 4;  // words of a row of the join
   static constexpr uint32_t kOutBytes = kTeams * 16 * kOutStride * 4;
-  static constexpr uint32_t kTileBytes = kQueryBytes + kBuffers * kExchange;
+  static constexpr uint32_t kTileBytes = kQueryBytes + kExchangeBytes;
   static constexpr uint32_t kShared = kTileBytes > kOutBytes ? kTileBytes : kOutBytes;
 };
 
@@ -149,9 +171,9 @@ __device__ __forceinline__ void block_work(const Outputs& o, uint32_t& unit, uin
 template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT>
 __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Outputs o) {
   using S = Shape<T, DW, VS, RT>;
-  constexpr uint32_t kThreads = 64 * S::kWaves, kRound = T::kSlots * S::kTeams;
+  constexpr uint32_t kThreads = 64 * S::kWaves, kRound = S::kRound;
   extern __shared__ __attribute__((aligned(16))) uint8_t shared[];
-  __shared__ float row_m[S::kTeams][RT * 16], row_l[S::kTeams][RT * 16];
+  __shared__ float row_m[S::kSets][RT * 16], row_l[S::kSets][RT * 16];
   __shared__ float2 row_sum[RT * 16];
   __shared__ uint32_t row_top[RT * 16], last_share;
   const CacheView& c = a.cache;
@@ -196,13 +218,14 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     seen_slots(length, t_last - 1u, c.capacity, a.window, all_lo, any_hi);
   }
   const uint32_t hi = min(c1, any_hi);
-  const uint32_t first = c0 + team * T::kSlots;
+  const uint32_t first = c0 + team * S::kTeamSlots;
 
   // Where a tile's rows lie, in two steps, so that the page numbers are there
   // before the rows are wanted.  FAST: of each score tile; else lane l has slot
   // l % kSlots.
+  constexpr uint32_t kPlaces = FAST ? S::kTeamTiles * S::kSubs : 1;
   struct Place {
-    uint32_t at[FAST ? S::kSubs : 1];
+    uint32_t at[kPlaces];
   };
   const uint32_t* table = c.table + (size_t)seq * c.max_pages;
   uint32_t bad = 0u;
@@ -210,7 +233,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     Place p;
     if constexpr (FAST) {
 #pragma unroll
-      for (uint32_t s = 0; s < S::kSubs; ++s) {
+      for (uint32_t s = 0; s < kPlaces; ++s) {
         const uint32_t slot = base + s * 16u;
         p.at[s] = slot < hi ? table[divided(slot, c.div_mul, c.div_shift)] : kNone;
       }
@@ -223,7 +246,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
   const auto rows_of = [&](uint32_t base, const Place& page) {
     Place p;
 #pragma unroll
-    for (uint32_t s = 0; s < (FAST ? S::kSubs : 1u); ++s) {
+    for (uint32_t s = 0; s < kPlaces; ++s) {
       const uint32_t slot = base + (FAST ? s * 16u : lane & (T::kSlots - 1u));
       p.at[s] = kNone;
       if (slot < hi) {
@@ -236,14 +259,14 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     }
     return p;
   };
-  // The slots that have a row, a bit each.  (FAST: and those behind the last
-  // on its page, which no row of the queries sees.)
-  const auto slots_there = [&](const Place& p) {
+  // The slots of tile `tile` that have a row, a bit each.  (FAST: and those behind
+  // the last on its page, which no row of the queries sees.)
+  const auto slots_there = [&](const Place& p, uint32_t tile) {
     if constexpr (!FAST) return (uint32_t)__builtin_amdgcn_ballot_w64(p.at[0] != kNone);
     uint32_t bits = 0u;
 #pragma unroll
     for (uint32_t s = 0; s < (FAST ? S::kSubs : 1u); ++s)
-      bits |= p.at[s] != kNone ? 0xffffu << (16u * s) : 0u;
+      bits |= p.at[tile * S::kSubs + s] != kNone ? 0xffffu << (16u * s) : 0u;
     return bits;
   };
   // Row `from` of score tile `sub`; a slot without a row reads the pool's first
@@ -257,24 +280,34 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       return base + (size_t)(at == kNone ? 0u : at) * row_bytes;
     }
   };
-  u32x4 key[S::kSubs][S::kSteps];
+  // (by slots: the wave's score tile in place of the first)
+  const auto own_place = [&](const Place& p) {
+    Place r = p;
+    if constexpr (S::kBySlots)
+#pragma unroll
+      for (uint32_t u = 1; u < VS; ++u)
+        if (half == u) r.at[0] = p.at[u];
+    return r;
+  };
+  u32x4 key[S::kOwnSubs][S::kKeySteps];
   const auto load_keys = [&](const Place& row) {
+    const Place own = own_place(row);
 #pragma unroll
-    for (uint32_t s = 0; s < S::kSubs; ++s) {
-      const uint8_t* p = pointer(keys, row, s, n);
+    for (uint32_t s = 0; s < S::kOwnSubs; ++s) {
+      const uint8_t* p = pointer(keys, own, s, n);
 #pragma unroll
-      for (uint32_t k = 0; k < S::kSteps; ++k) {
-        uint32_t at = ((half * S::kSteps + k) * 4u + j) * 16u;
+      for (uint32_t k = 0; k < S::kKeySteps; ++k) {
+        uint32_t at = (((S::kBySlots ? 0u : half * S::kSteps) + k) * 4u + j) * 16u;
         if (!FAST) at = min(at, row_bytes - 16u);  // (its query values are 0)
         key[s][k] = *reinterpret_cast<const Words4*>(p + at);
       }
     }
   };
-  uint32_t value[S::kRows][S::kPasses][S::kWords];
-  const auto load_values = [&](const Place& row) {
+  uint32_t value[S::kTeamTiles][S::kRows][S::kPasses][S::kWords];
+  const auto load_values = [&](const Place& row, uint32_t tile) {
 #pragma unroll
     for (uint32_t i = 0; i < S::kRows; ++i) {
-      const uint8_t* p = pointer(values, row, i / 4u, j * 4u + i % 4u);
+      const uint8_t* p = pointer(values, row, tile * S::kSubs + i / 4u, j * 4u + i % 4u);
 #pragma unroll
       for (uint32_t u = 0; u < S::kPasses; ++u) {
         uint32_t at = ((half * S::kPasses + u) * 16u + n) * (S::kWords * 4u);
@@ -282,11 +315,11 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
         if constexpr (S::kWords == 4) {
           const u32x4 w = *reinterpret_cast<const Words4*>(p + at);
 #pragma unroll
-          for (uint32_t x = 0; x < 4; ++x) value[i][u][x] = w[x];
+          for (uint32_t x = 0; x < 4; ++x) value[tile][i][u][x] = w[x];
         } else {
           const Words2 w = *reinterpret_cast<const Words2*>(p + at);
-          value[i][u][0] = w.x;
-          value[i][u][1] = w.y;
+          value[tile][i][u][0] = w.x;
+          value[tile][i][u][1] = w.y;
         }
       }
     }
@@ -380,7 +413,8 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     }
   }
   if (!S::kInRegisters) exchange_barrier();
-  load_values(row);
+#pragma unroll
+  for (uint32_t u = 0; u < S::kTeamTiles; ++u) load_values(row, u);
 
   // ---- the lane's rows, and their slots
   uint32_t begin[RT], end[RT];
@@ -407,8 +441,9 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     for (uint32_t d = 0; d < S::kTiles; ++d) out[i][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // out^T += V^T p^T with the values in `value`
-  const auto add_values = [&](const float (&p)[RT][S::kRows]) {
+  // out^T += V^T p^T with a tile's values
+  const auto add_values = [&](uint32_t tile, const u32x4 (&b)[RT][T::kPieces]) {
+    const auto& v = value[tile];
     if constexpr (S::kWide) {
 #pragma unroll
       for (uint32_t u = 0; u < S::kPasses; ++u)
@@ -419,29 +454,20 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
             for (uint32_t r = 0; r < RT; ++r)
               out[r][u * S::kEach + d] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  __uint_as_float(value[i][u][d]), p[r][i], out[r][u * S::kEach + d], 0, 0, 0);
+                  __uint_as_float(v[i][u][d]), __uint_as_float(b[r][0][i]),
+                  out[r][u * S::kEach + d], 0, 0, 0);
     } else {
-      u32x4 b[RT][T::kPieces];
-#pragma unroll
-      for (uint32_t r = 0; r < RT; ++r)
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i += 2) {
-          uint32_t w[T::kPieces];
-          T::split(p[r][i], p[r][i + 1], w);
-#pragma unroll
-          for (uint32_t k = 0; k < T::kPieces; ++k) b[r][k][i / 2] = w[k];
-        }
       // (four sums at a time, so that none waits for the one before)
 #pragma unroll
       for (uint32_t u = 0; u < S::kPasses; ++u)
 #pragma unroll
         for (uint32_t d = 0; d < S::kEach; d += 4) {
-          u32x4 v[4];
+          u32x4 x[4];
 #pragma unroll
           for (uint32_t e = 0; e < 4; ++e)
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
-              v[e][i] = perm(value[2 * i + 1][u][(d + e) / 2], value[2 * i][u][(d + e) / 2],
+              x[e][i] = perm(v[2 * i + 1][u][(d + e) / 2], v[2 * i][u][(d + e) / 2],
                              e & 1 ? kHighs : kLows);
 #pragma unroll
           for (uint32_t r = 0; r < RT; ++r)
@@ -450,9 +476,68 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
               for (uint32_t e = 0; e < 4; ++e) {
                 f32x4& acc = out[r][u * S::kEach + d + e];
-                acc = T::mfma(v[e], b[r][k], acc);
+                acc = T::mfma(x[e], b[r][k], acc);
               }
         }
+    }
+  };
+  // p of a lane's slots, as the words of the B operands that they make
+  const auto operands = [&](const float (&p)[S::kOwnRows], uint32_t (&b)[T::kPieces][4]) {
+    if constexpr (S::kWide) {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) b[0][i] = __float_as_uint(p[i]);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < S::kOwnRows; i += 2) {
+        uint32_t w[T::kPieces];
+        T::split(p[i], p[i + 1], w);
+#pragma unroll
+        for (uint32_t k = 0; k < T::kPieces; ++k) b[k][i / 2] = w[k];
+      }
+    }
+  };
+  // A slot that no row sees may hold anything: its values are taken as 0.  So
+  // are those of a slot with a value that is no finite number, where not all
+  // rows see it, for 0 times that would reach the others; the rows that do
+  // see it are none from then on.
+  const auto clear_unseen = [&](uint32_t tile, uint32_t base, uint32_t there) {
+    constexpr uint32_t kAll = T::kSlots == 32u ? 0xffffffffu : 0xffffu;
+    if ((slot_bits(all_lo, all_hi, base) & there & kAll) == kAll) return;
+    auto& v = value[tile];
+    const uint32_t used = (slot_bits(any_lo, any_hi, base) & there) >> (4u * j);
+    uint32_t lost = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < S::kRows; ++i) {
+      const uint32_t at = i / 4u * 16u + i % 4u;
+      bool use = (used >> at & 1u) != 0u;
+      uint32_t odd = 0u;
+#pragma unroll
+      for (uint32_t u = 0; u < S::kPasses; ++u)
+#pragma unroll
+        for (uint32_t w = 0; w < S::kWords; ++w) odd |= (v[i][u][w] & T::kExponent) + T::kUnit;
+      const uint64_t odds = __builtin_amdgcn_ballot_w64((odd & T::kCarry) != 0u);
+      if ((odds >> (16u * j) & 0xffffu) != 0u) {  // (16 lanes have the slot's values)
+#pragma unroll
+        for (uint32_t r = 0; r < RT; ++r) {
+          const uint32_t seen = (slot_bits(begin[r], end[r], base) & there) >> (4u * j);
+          lost |= (seen >> at & 1u) << r;
+        }
+        use = false;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < S::kPasses; ++u)
+#pragma unroll
+        for (uint32_t w = 0; w < S::kWords; ++w) v[i][u][w] = use ? v[i][u][w] : 0u;
+    }
+    if (__builtin_amdgcn_ballot_w64(lost != 0u)) {
+      lost |= __shfl_xor(lost, 16, 64);
+      lost |= __shfl_xor(lost, 32, 64);
+#pragma unroll
+      for (uint32_t r = 0; r < RT; ++r) {
+        const float none = lost >> r & 1u ? NAN : 0.0f;
+#pragma unroll
+        for (uint32_t d = 0; d < S::kTiles; ++d) out[r][d] += none;
+      }
     }
   };
 
@@ -460,20 +545,23 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
   // others', meet at the exchange)
   uint32_t turn = 0u;
   for (uint32_t at = c0; at < hi; at += kRound) {
-    const uint32_t base = at + team * T::kSlots;
-    const uint32_t there = slots_there(row);
-    next_page = pages_of(base + 2u * kRound);
+    const uint32_t team_base = at + team * S::kTeamSlots;
+    const uint32_t base = team_base + (S::kBySlots ? half * 16u : 0u);  // of the wave's scores
+    uint32_t there[S::kTeamTiles];
+#pragma unroll
+    for (uint32_t u = 0; u < S::kTeamTiles; ++u) there[u] = slots_there(row, u);
+    const uint32_t own_there = S::kBySlots ? (own_place(row).at[0] != kNone ? 0xffffu : 0u) : there[0];
+    next_page = pages_of(team_base + 2u * kRound);
     // ---- scores
-    f32x4 sum[RT][S::kSubs];
+    f32x4 sum[RT][S::kOwnSubs];
     // (queries in LDS are read for each tile: kept across tiles, they would not leave
     // registers for it; a step's are under way while the one before is multiplied)
-    uint32_t q_at = half * S::kSteps * 64u + lane;
+    uint32_t q_at = (S::kBySlots ? 0u : half * S::kSteps * 64u) + lane;
     asm volatile("" : "+v"(q_at));
     const auto read_query = [&](uint32_t i, u32x4(&q)[T::kPieces]) {
       if constexpr (!S::kInRegisters)
 #pragma unroll
-        for (uint32_t w = 0; w < T::kPieces; ++w)
-          q[w] = q_lds[w * S::kItems + (i / S::kSteps * VS * S::kSteps + i % S::kSteps) * 64u + q_at];
+        for (uint32_t w = 0; w < T::kPieces; ++w) q[w] = q_lds[w * S::kItems + i * 64u + q_at];
       else
 #pragma unroll
         for (uint32_t w = 0; w < T::kPieces; ++w) q[w] = query[i][w];
@@ -484,15 +572,15 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     for (uint32_t r = 0; r < RT; ++r) {
       // sums that do not wait for each other: two of the f32 instructions, one a piece else
       constexpr uint32_t kSums = S::kWide ? 2 : T::kPieces;
-      f32x4 piece[S::kSubs][kSums];
+      f32x4 piece[S::kOwnSubs][kSums];
 #pragma unroll
-      for (uint32_t s = 0; s < S::kSubs; ++s)
+      for (uint32_t s = 0; s < S::kOwnSubs; ++s)
 #pragma unroll
         for (uint32_t k = 0; k < kSums; ++k) piece[s][k] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (uint32_t k = 0; k < S::kSteps; ++k) {
-        const uint32_t i = r * S::kSteps + k;
-        if (i + 1u < RT * S::kSteps) read_query(i + 1u, q[(i + 1u) & 1u]);
+      for (uint32_t k = 0; k < S::kKeySteps; ++k) {
+        const uint32_t i = r * S::kKeySteps + k;
+        if (i + 1u < RT * S::kKeySteps) read_query(i + 1u, q[(i + 1u) & 1u]);
         if (!S::kInRegisters) __builtin_amdgcn_sched_barrier(0);
         const auto& now = q[i & 1u];
         if constexpr (S::kWide) {
@@ -504,12 +592,12 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
           for (uint32_t w = 0; w < T::kPieces; ++w)
 #pragma unroll
-            for (uint32_t s = 0; s < S::kSubs; ++s)
+            for (uint32_t s = 0; s < S::kOwnSubs; ++s)
               piece[s][w] = T::mfma(key[s][k], now[w], piece[s][w]);
         }
       }
 #pragma unroll
-      for (uint32_t s = 0; s < S::kSubs; ++s) {
+      for (uint32_t s = 0; s < S::kOwnSubs; ++s) {
         sum[r][s] = piece[s][kSums - 1];
 #pragma unroll
         for (int k = (int)kSums - 2; k >= 0; --k) sum[r][s] += piece[s][k];
@@ -518,111 +606,120 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     }
     __builtin_amdgcn_sched_barrier(0);
     // ---- the next tile's keys
-    row = rows_of(base + kRound, page);
+    row = rows_of(team_base + kRound, page);
     page = next_page;
     load_keys(row);  // (behind the last tile too: a condition would hold both sets of registers)
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (VS == 2) {
+    if constexpr (VS > 1 && !S::kBySlots) {
       // ---- the other half's scores: both waves add the first half's to the second's
       f32x4* place = reinterpret_cast<f32x4*>(shared + S::kQueryBytes) +
-                     (turn % S::kBuffers) * (S::kExchange / 16u);
-      if (S::kBuffers == 1u) exchange_barrier();  // (the last ones are taken)
+                     (turn & 1u) * (S::kHalves / 16u);
 #pragma unroll
-      for (uint32_t r = 0; r < RT; ++r)
-#pragma unroll
-        for (uint32_t s = 0; s < S::kSubs; ++s)
-          place[((wave * RT + r) * S::kSubs + s) * 64u + lane] = sum[r][s];
+      for (uint32_t s = 0; s < S::kSubs; ++s)
+        place[(wave * S::kSubs + s) * 64u + lane] = sum[0][s];
       exchange_barrier();
 #pragma unroll
-      for (uint32_t r = 0; r < RT; ++r)
-#pragma unroll
-        for (uint32_t s = 0; s < S::kSubs; ++s)
-          sum[r][s] += place[(((wave ^ 1u) * RT + r) * S::kSubs + s) * 64u + lane];
+      for (uint32_t s = 0; s < S::kSubs; ++s)
+        sum[0][s] += place[((wave ^ 1u) * S::kSubs + s) * 64u + lane];
       ++turn;
     }
     // ---- p
-    float p[RT][S::kRows];
-    uint32_t seen[RT];  // bits 0..3 and 16..19: the row sees the lane's slots
+    float p[RT][S::kOwnRows], now[RT];
 #pragma unroll
     for (uint32_t r = 0; r < RT; ++r) {
+      // bits 0..3 and 16..19: the row sees the lane's slots
+      const uint32_t seen = (slot_bits(begin[r], end[r], base) & own_there) >> (4u * j) &
+                            (S::kOwnSubs == 2u ? 0x000f000fu : 0xfu);
       float top = -INFINITY;
-      seen[r] = (slot_bits(begin[r], end[r], base) & there) >> (4u * j) &
-                (T::kSlots == 32u ? 0x000f000fu : 0xfu);
 #pragma unroll
-      for (uint32_t i = 0; i < S::kRows; ++i) {
-        p[r][i] = seen[r] >> (i / 4u * 16u + i % 4u) & 1u ? sum[r][i / 4u][i % 4u] : -INFINITY;
+      for (uint32_t i = 0; i < S::kOwnRows; ++i) {
+        p[r][i] = seen >> (i / 4u * 16u + i % 4u) & 1u ? sum[r][i / 4u][i % 4u] : -INFINITY;
         top = fmaxf(top, p[r][i]);
       }
-      any |= seen[r] ? 1u << r : 0u;
-      if (score_row[r] && half == 0u) {
+      any |= seen ? 1u << r : 0u;
+      if (score_row[r] && (S::kBySlots || half == 0u)) {
 #pragma unroll
-        for (uint32_t s = 0; s < S::kSubs; ++s) {
+        for (uint32_t s = 0; s < S::kOwnSubs; ++s) {
           const uint32_t slot = base + s * 16u + j * 4u;
           if (slot < o.score_stride)
             *reinterpret_cast<float4*>(score_row[r] + slot) =
                 make_float4(p[r][4 * s], p[r][4 * s + 1], p[r][4 * s + 2], p[r][4 * s + 3]);
         }
       }
-      const float now = fmaxf(m[r], columns_max(top));
-      const float from = now == -INFINITY ? 0.0f : now - T::kShift;
-      if (__builtin_amdgcn_ballot_w64(now > m[r])) {
-        const float keep = m[r] == -INFINITY ? 0.0f : exp2_of(m[r] - now);
+      now[r] = columns_max(top);
+      if (S::kBySlots && j == 0u) row_m[wave][r * 16u + n] = now[r];
+    }
+    if constexpr (S::kBySlots) {  // the team's maxima (and the last round's p is read)
+      exchange_barrier();
+#pragma unroll
+      for (uint32_t r = 0; r < RT; ++r)
+#pragma unroll
+        for (uint32_t u = 0; u < VS; ++u) now[r] = fmaxf(now[r], row_m[team * VS + u][r * 16u + n]);
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < RT; ++r) {
+      now[r] = fmaxf(m[r], now[r]);
+      const float from = now[r] == -INFINITY ? 0.0f : now[r] - T::kShift;
+      if (__builtin_amdgcn_ballot_w64(now[r] > m[r])) {
+        const float keep = m[r] == -INFINITY ? 0.0f : exp2_of(m[r] - now[r]);
         l[r] *= keep;
 #pragma unroll
         for (uint32_t d = 0; d < S::kTiles; ++d) out[r][d] *= keep;
-        m[r] = now;
+        m[r] = now[r];
       }
 #pragma unroll
-      for (uint32_t i = 0; i < S::kRows; ++i) {
+      for (uint32_t i = 0; i < S::kOwnRows; ++i) {
         p[r][i] = exp2_of(p[r][i] - from);  // (0 where not seen)
         l[r] += p[r][i];
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     // ---- out
-    // A slot that no row sees may hold anything: its values are taken as 0.  So
-    // are those of a slot with a value that is no finite number, where not all
-    // rows see it, for 0 times that would reach the others; the rows that do
-    // see it are none from then on.
-    constexpr uint32_t kAll = T::kSlots == 32u ? 0xffffffffu : 0xffffu;
-    if ((slot_bits(all_lo, all_hi, base) & there & kAll) != kAll) {
-      const uint32_t used = (slot_bits(any_lo, any_hi, base) & there) >> (4u * j);
-      uint32_t lost = 0u;
+    if constexpr (S::kBySlots) {
+      // each wave's p into the team's operands: a tile's slots are those of one or two waves
+      constexpr uint32_t kPart = 4u / S::kSubs;  // words
+      uint32_t* place = reinterpret_cast<uint32_t*>(shared + S::kQueryBytes);
 #pragma unroll
-      for (uint32_t i = 0; i < S::kRows; ++i) {
-        const uint32_t at = i / 4u * 16u + i % 4u;
-        bool use = (used >> at & 1u) != 0u;
-        uint32_t odd = 0u;
+      for (uint32_t r = 0; r < RT; ++r) {
+        uint32_t b[T::kPieces][4];
+        operands(p[r], b);
 #pragma unroll
-        for (uint32_t u = 0; u < S::kPasses; ++u)
-#pragma unroll
-          for (uint32_t w = 0; w < S::kWords; ++w)
-            odd |= (value[i][u][w] & T::kExponent) + T::kUnit;
-        const uint64_t odds = __builtin_amdgcn_ballot_w64((odd & T::kCarry) != 0u);
-        if ((odds >> (16u * j) & 0xffffu) != 0u) {  // (16 lanes have the slot's values)
-#pragma unroll
-          for (uint32_t r = 0; r < RT; ++r) lost |= (seen[r] >> at & 1u) << r;
-          use = false;
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < S::kPasses; ++u)
-#pragma unroll
-          for (uint32_t w = 0; w < S::kWords; ++w) value[i][u][w] = use ? value[i][u][w] : 0u;
-      }
-      if (__builtin_amdgcn_ballot_w64(lost != 0u)) {
-        lost |= __shfl_xor(lost, 16, 64);
-        lost |= __shfl_xor(lost, 32, 64);
-#pragma unroll
-        for (uint32_t r = 0; r < RT; ++r) {
-          const float none = lost >> r & 1u ? NAN : 0.0f;
-#pragma unroll
-          for (uint32_t d = 0; d < S::kTiles; ++d) out[r][d] += none;
+        for (uint32_t k = 0; k < T::kPieces; ++k) {
+          uint32_t* to = place + ((((team * S::kTeamTiles + half / S::kSubs) * RT + r) * T::kPieces + k) * 64u + lane) * 4u +
+                         half % S::kSubs * kPart;
+          if constexpr (kPart == 4u) *reinterpret_cast<uint4*>(to) = make_uint4(b[k][0], b[k][1], b[k][2], b[k][3]);
+          else *reinterpret_cast<uint2*>(to) = make_uint2(b[k][0], b[k][1]);
         }
       }
+      exchange_barrier();
+#pragma unroll
+      for (uint32_t u = 0; u < S::kTeamTiles; ++u) {
+        u32x4 b[RT][T::kPieces];
+#pragma unroll
+        for (uint32_t r = 0; r < RT; ++r)
+#pragma unroll
+          for (uint32_t k = 0; k < T::kPieces; ++k)
+            b[r][k] = reinterpret_cast<const u32x4*>(
+                place)[(((team * S::kTeamTiles + u) * RT + r) * T::kPieces + k) * 64u + lane];
+        clear_unseen(u, team_base + u * T::kSlots, there[u]);
+        add_values(u, b);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(row, u);  // the next tile's
+      }
+    } else {
+      u32x4 b[RT][T::kPieces];
+#pragma unroll
+      for (uint32_t r = 0; r < RT; ++r) {
+        uint32_t w[T::kPieces][4];
+        operands(p[r], w);
+#pragma unroll
+        for (uint32_t k = 0; k < T::kPieces; ++k) b[r][k] = u32x4{w[k][0], w[k][1], w[k][2], w[k][3]};
+      }
+      clear_unseen(0u, base, own_there);
+      add_values(0u, b);
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(row, 0u);  // the next tile's
     }
-    add_values(p);
-    __builtin_amdgcn_sched_barrier(0);
-    load_values(row);  // the next tile's
   }
   if (bad) report_device_error(a.report, kDevErrCachePage);
 
@@ -636,9 +733,9 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
     if (l[r] == 0.0f && m[r] == -INFINITY && (any >> r & 1u) != 0u) l[r] = -1.0f;
-    if (j == 0u && half == 0u) {
-      row_m[team][r * 16u + n] = m[r];
-      row_l[team][r * 16u + n] = l[r];
+    if (j == 0u && (S::kBySlots || half == 0u)) {
+      row_m[S::kBySlots ? wave : team][r * 16u + n] = m[r];
+      row_l[S::kBySlots ? wave : team][r * 16u + n] = l[r];
     }
   }
   float* join = reinterpret_cast<float*>(shared) + (team * 16u + n) * S::kOutStride;
@@ -647,11 +744,11 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
     exchange_barrier();  // (the queries and scores, or the last tile's outputs, are no longer read)
     float top = -INFINITY;
 #pragma unroll
-    for (uint32_t w = 0; w < S::kTeams; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
+    for (uint32_t w = 0; w < S::kSets; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
     if (wave == 0u) {
       Joined sum_l;
 #pragma unroll
-      for (uint32_t w = 0; w < S::kTeams; ++w)
+      for (uint32_t w = 0; w < S::kSets; ++w)
         sum_l.add(make_float2(row_m[w][r * 16u + n], row_l[w][r * 16u + n]), top);
       if (j == 0u) row_sum[r * 16u + n] = sum_l.result(top);
     }
@@ -777,7 +874,7 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   if (attr != hipSuccess) return attr;
   const uint32_t tiles = row_tiles(a.tokens, a.group);
   o.tile_groups = (tiles + RT - 1u) / RT;
-  o.round = T::kSlots * S::kTeams;
+  o.round = S::kRound;
   o.shift = T::kShift;
   o.shares = shares_for(a.cache, o.tile_groups, o.round);
   o.by_shares = divisor_of(o.shares);
@@ -796,25 +893,30 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   return launch_attention_join(a, o, s);
 }
 
-// The row tiles a wave takes, so that the cache is read for several at once:
-// as many as leave registers for two waves a SIMD beside the tile, three of an
-// f32 cache, two else.
-template <typename T, uint32_t DW, uint32_t VS>
+// The row tiles a workgroup takes, so that the cache is read for several at
+// once: two, or three where two would leave the last group one of its two; of
+// heads of 128 in 16 bits two, for three of them do not fit the registers (80
+// us instead of 59 for 44 rows over 44,236 slots of 8 heads).  Heads of 256
+// are shared by slots: 48 rows over 44,236 slots of 4 heads 54 us, three tiles
+// at once, where two waves with half of the head each and two tiles at once
+// took 64.
+template <typename T, uint32_t DIM>
 hipError_t launch_rows(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
   const uint32_t tiles = row_tiles(a.tokens, a.group);
-  if (tiles == 1u) return launch_mfma<T, DW, VS, true, 1>(a, o, s);
-  if constexpr (T::kBytes == 4)
-    if (tiles == 3u || tiles > 4u) return launch_mfma<T, DW, VS, true, 3>(a, o, s);
-  return launch_mfma<T, DW, VS, true, 2>(a, o, s);
+  if (tiles == 1u) return launch_mfma<T, (DIM < 128 ? DIM : 128), (DIM + 127) / 128, true, 1>(a, o, s);
+  constexpr uint32_t kDw = DIM == 256 ? 64 : DIM, kVs = DIM / kDw;
+  if constexpr (DIM != 128 || T::kBytes == 4)
+    if (tiles == 3u || tiles > 4u) return launch_mfma<T, kDw, kVs, true, 3>(a, o, s);
+  return launch_mfma<T, kDw, kVs, true, 2>(a, o, s);
 }
 
 template <typename T>
 hipError_t launch_type(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
   const uint32_t dim = a.cache.head_dim;
   if (a.cache.page_tokens % 16u == 0u) {
-    if (dim == 64u) return launch_rows<T, 64, 1>(a, o, s);
-    if (dim == 128u) return launch_rows<T, 128, 1>(a, o, s);
-    if (dim == 256u) return launch_rows<T, 128, 2>(a, o, s);
+    if (dim == 64u) return launch_rows<T, 64>(a, o, s);
+    if (dim == 128u) return launch_rows<T, 128>(a, o, s);
+    if (dim == 256u) return launch_rows<T, 256>(a, o, s);
   }
   if (dim <= 64u) return launch_mfma<T, 64, 1, false, 1>(a, o, s);
   if (dim <= 128u) return launch_mfma<T, 128, 1, false, 1>(a, o, s);

@@ -83,7 +83,7 @@ hipError_t launch_attention_mfma(const AttentionArgs& a, const Space& sp, bool* 
   const uint32_t row = c.head_dim * (c.type == kKvF32 ? 4u : 2u);
   *taken = row % 16u == 0u && aligned4(c.keys) && aligned4(c.values);
   // (the rounds of all sequences are counted in 31 bits)
-  *taken = *taken && (uint64_t)c.sequences * (c.capacity / 64u + 3u) < 0x7fffffffu;
+  *taken = *taken && (uint64_t)c.sequences * (c.capacity / 32u + 3u) < 0x7fffffffu;
   if (!*taken) return hipSuccess;
   uint8_t* w = static_cast<uint8_t*>(a.workspace);
   Outputs o{};
