@@ -140,13 +140,14 @@ def test_alignments_and_strides(hip_ctx, dev, kind, dim, offset):
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_numbers_in_unseen_slots_do_not_matter(hip_ctx, dev, kind, dim):
+@pytest.mark.parametrize("heads", [4, 10, 16])  # one, two and three row tiles
+def test_numbers_in_unseen_slots_do_not_matter(hip_ctx, dev, kind, dim, heads):
     """NaN and infinities behind the sequence, before the window, in later new
     tokens' rows for the earlier ones, and on pages of nobody."""
     rng = np.random.default_rng(dim)
     lengths, tokens, window = [0, 21, 90, 150], 6, 40
     c = R.Cache(dev, rng, kind, 4, 2, dim, 16, 11, lengths)
-    clean = R.attention(c, q := rng.standard_normal((4, tokens, 4, dim)).astype(np.float32),
+    clean = R.attention(c, q := rng.standard_normal((4, tokens, heads, dim)).astype(np.float32),
                         float(np.float32(dim ** -0.5)), window, None)
     seen = np.zeros(c.keys.shape[:3:2], bool)  # [page][place]
     for s, n in enumerate(lengths):
