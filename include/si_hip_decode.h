@@ -134,11 +134,13 @@ int si_hip_kv_advance_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
  * q_head_stride; d_out contiguous [sequences][tokens][heads][head_dim].  A row
  * with nothing to attend to (t >= d_counts[s], slots on pages beyond the pool)
  * is zeros.  Slots that a row does not see have no part in it, whatever they
- * hold; a value in them that is no number does not reach it.
+ * hold: NaN and infinities in them do not reach it.  A row that sees a key or
+ * value that is no finite number is not a number, in part or as a whole.
  *
  * With d_weights, [sequences][kv_heads][weights_stride], entry i of kv head h
  * grows by the sum of p_i over the head's query heads and the new tokens;
- * weights_stride is at least the capacity.
+ * weights_stride is at least the capacity.  Entries of slots that a later call
+ * fills anew (refused drafts') are the caller's to clear.
  *
  * d_workspace: si_hip_paged_attention_workspace() bytes of 16-byte aligned
  * device memory that this call may write until it has run. */

@@ -30,7 +30,8 @@ bool product(size_t a, size_t b, size_t *out) { return !__builtin_mul_overflow(a
 int check_cache(const si_hip_kv_cache *c, CacheView *view) {
   if (!c) return set_error(SI_HIP_ERR_NULL, "key-value cache is null");
   if (c->ggml_type != kKvF32 && c->ggml_type != kKvF16 && c->ggml_type != kKvBF16)
-    return set_error(SI_HIP_ERR_UNSUPPORTED_TYPE, "unsupported key-value cache type %u", c->ggml_type);
+    return set_error(SI_HIP_ERR_UNSUPPORTED_TYPE, "unsupported key-value cache type %u",
+                     c->ggml_type);
   if (c->kv_heads == 0 || c->head_dim == 0 || c->head_dim > SI_HIP_MAX_HEAD_DIM ||
       c->page_tokens == 0 || c->pages == 0 || c->sequences == 0 || c->max_pages == 0)
     return set_error(SI_HIP_ERR_DIMENSIONS, "key-value cache dimensions are invalid");

@@ -103,7 +103,9 @@ struct Span {
 };
 
 // A value that all lanes hold, in a scalar register.
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return __builtin_amdgcn_readfirstlane(v);
+}
 
 // Running sums of the first `count` lanes' values.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_t count) {
