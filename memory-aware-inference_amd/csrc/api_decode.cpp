@@ -86,6 +86,15 @@ int check_heads(const CacheView &v, size_t heads) {
   return SI_HIP_OK;
 }
 
+// The kept scores of a call with weights: a row of slots for each row of queries.
+int check_scores(const CacheView &v, size_t heads, size_t tokens) {
+  size_t n;
+  if (!product((size_t)v.sequences * heads * tokens, (size_t)v.capacity + 3u, &n) ||
+      n > SIZE_MAX / 16)
+    return set_error(SI_HIP_ERR_OVERFLOW, "attention weights exceed HIP limits");
+  return SI_HIP_OK;
+}
+
 // Rows of heads a stride apart hold `heads` heads of `dim` values each.
 int check_strides(size_t token_stride, size_t head_stride, size_t heads, size_t dim,
                   const char *what) {
@@ -217,7 +226,7 @@ size_t si_hip_paged_attention_workspace(const si_hip_kv_cache *cache, size_t hea
                                         int with_weights) {
   CacheView view;
   if (check_cache(cache, &view) || check_step(view, tokens, SI_HIP_MAX_STEP_TOKENS, "attention") ||
-      check_heads(view, heads))
+      check_heads(view, heads) || (with_weights && check_scores(view, heads, tokens)))
     return 0;
   clear_error();
   return attention_workspace_bytes(view, (uint32_t)heads, (uint32_t)tokens, with_weights != 0);
@@ -238,6 +247,7 @@ int si_hip_paged_attention_device(si_hip_context *ctx, const si_hip_kv_cache *ca
     return rc;
   if (!std::isfinite(scale))
     return set_error(SI_HIP_ERR_DIMENSIONS, "attention scale is not finite");
+  if (d_weights && (rc = check_scores(a.cache, heads, tokens)) != 0) return rc;
   if (d_weights && weights_stride < a.cache.capacity)
     return set_error(SI_HIP_ERR_DIMENSIONS, "attention weights are shorter than the capacity");
   if (workspace_bytes < attention_workspace_bytes(a.cache, (uint32_t)heads, (uint32_t)tokens,

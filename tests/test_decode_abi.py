@@ -110,6 +110,16 @@ def test_attention_refusals():
     assert si_hip.lib().si_hip_paged_attention_workspace(cache(), 6, 1, 0) == 0
 
 
+def test_attention_scores_beyond_the_address_space():
+    """Sizes whose product wraps to a small workspace."""
+    c = cache(sequences=65535, kv_heads=1, max_pages=(1 << 26) + 1, head_dim=1)
+    lib = si_hip.lib()
+    assert lib.si_hip_paged_attention_workspace(c, 65535, 16, 1) == 0
+    assert "attention weights" in si_hip.last_error()
+    assert attend(c, heads=65535, tokens=16, qs=65535, qh=1, w=P, ws=1 << 31) == OVER
+    assert lib.si_hip_paged_attention_workspace(c, 65535, 16, 0) > 0
+
+
 def test_evict_refusals():
     assert evict(keep=0) == DIM and evict(keep=65) == DIM
     assert evict(sinks=17) == DIM and evict(sinks=8, recent=9) == DIM
