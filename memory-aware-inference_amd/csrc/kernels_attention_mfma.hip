@@ -15,7 +15,8 @@ constexpr uint32_t kThreads = 512;
 __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outputs o) {
   __shared__ float4 shared[kThreads];
   const CacheView& c = a.cache;
-  const uint32_t rows = a.tokens * a.group, head = blockIdx.x, kv = head / rows, r = head - kv * rows;
+  const uint32_t rows = a.tokens * a.group, head = blockIdx.x, kv = head / rows;
+  const uint32_t r = head - kv * rows;
   const uint32_t seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63u;
   // the rounds before the sequence's, and its own
   uint32_t before = 0u, total = 0u;
@@ -34,6 +35,23 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
   const uint32_t shares = (first + span_of(a, seq, o.round).rounds - 1u) / deal.each - share0 + 1u;
   if (shares == 1u) return;  // written already
   const auto at = [&](uint32_t p) { return (size_t)(share0 + p + seq) * c.kv_heads * rows + head; };
+  // (the first of the thread's shares are under way while the maximum is found)
+  const uint32_t dim = c.head_dim, width = dim / 4u, groups = kThreads / width;
+  const uint32_t group = tid / width, d = (tid - group * width) * 4u;
+  constexpr uint32_t kAhead = 8;
+  float4 x[kAhead];
+  float x_m[kAhead];
+#pragma unroll
+  for (uint32_t k = 0; k < kAhead; ++k) {
+    const uint32_t p = group + k * groups;
+    if (k * groups >= shares) break;
+    x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    x_m[k] = -INFINITY;
+    if (group < groups && p < shares) {
+      x[k] = *reinterpret_cast<const float4*>(o.part_out + at(p) * dim + d);
+      x_m[k] = o.part_stats[at(p)].x;
+    }
+  }
   float top = -INFINITY;
   for (uint32_t p = lane; p < shares; p += 64u) top = fmaxf(top, o.part_stats[at(p)].x);
 #pragma unroll
@@ -44,12 +62,12 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
   for (int s = 32; s > 0; s >>= 1) sum_l.l += __shfl_xor(sum_l.l, s, 64);
   sum_l.minus = __builtin_amdgcn_ballot_w64(sum_l.minus) != 0u;
   const float2 st = sum_l.result(top);
-  const uint32_t dim = c.head_dim, width = dim / 4u, groups = kThreads / width;
-  const uint32_t group = tid / width, d = (tid - group * width) * 4u;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (group < groups) {
-#pragma unroll 4
-    for (uint32_t p = group; p < shares; p += groups) {
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k)
+      if (k * groups < shares) add_share(x_m[k], top, x[k], sum);
+    for (uint32_t p = group + kAhead * groups; p < shares; p += groups) {
       add_share(o.part_stats[at(p)].x, top,
                 *reinterpret_cast<const float4*>(o.part_out + at(p) * dim + d), sum);
     }
@@ -65,14 +83,15 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttentionArgs a, Outp
   float* to = a.out + (((size_t)seq * a.tokens + t) * a.heads + h) * dim + d;
   const float4 v = finished(sum, st);
   *reinterpret_cast<Floats4*>(to) = Floats4{v.x, v.y, v.z, v.w};
-  if (o.stats && tid == 0u) o.stats[(size_t)seq * c.kv_heads * rows + head] = row_stats(st, o.shift);
+  if (o.stats && tid == 0u)
+    o.stats[(size_t)seq * c.kv_heads * rows + head] = row_stats(st, o.shift);
 }
 
 }  // namespace
 
 hipError_t launch_attention_join(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
-  attention_join<<<dim3(a.cache.kv_heads * a.tokens * a.group, a.cache.sequences), kThreads, 0, s>>>(
-      a, o);
+  const dim3 grid(a.cache.kv_heads * a.tokens * a.group, a.cache.sequences);
+  attention_join<<<grid, kThreads, 0, s>>>(a, o);
   return hipGetLastError();
 }
 
