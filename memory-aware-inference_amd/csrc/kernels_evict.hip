@@ -3,15 +3,16 @@
 // Weights are compared as 32-bit integers whose order is theirs, so the
 // selection is exact and its ties are too: the `need`-th largest integer T of
 // the slots between the first `sinks` and the last `recent` is found digit by
-// digit from histograms in LDS, then the slots above T and the first ones
-// equal to it are kept.  A second kernel moves the kept rows; it is bound by
-// memory, the selection by the chain of its passes.  So a head's selection is
-// one workgroup's, whose threads read their slots, next to each other, once
-// and hold them (up to 32768 slots; more are read in each pass), and one scan
-// over the threads places all that is kept.  Measured: 4 heads of 4111 slots
-// of 256 values, 3001 kept, 17.4 us (selection 11, move 6) for 24.8 MB; 64 heads
-// of up to 16,384 slots of 128, 6144 kept, 94 us (17 and 77) for 379 MB, the
-// move at 4.9 TB/s read and written.
+// digit from histograms in LDS (as far as one bin holds both kept slots and
+// others), then the slots above T and the first ones equal to it are kept.  A
+// second kernel moves the kept rows; it is bound by memory, the selection by
+// the chain of its passes.  So a head's selection is one workgroup's, whose
+// threads read their slots, next to each other, once and hold them (up to 32768
+// slots; more are read in each pass), and one scan over the threads places all
+// that is kept.  Measured: 4 heads of 4111 slots of 256 values, 3001 kept,
+// 16.3 us (selection 9.5, move 6) for 24.8 MB; 64 heads of up to 16,384 slots of
+// 128, 6144 kept, 94 us (16 and 77) for 379 MB, the move at 4.9 TB/s read and
+// written.
 #include "decode_internal.h"
 
 namespace sihip {
@@ -54,7 +55,7 @@ __device__ __forceinline__ V block_scan(V v, V* part, V& total) {
 template <uint32_t HELD>
 __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
   __shared__ uint4 bins[2048];  // (four counts a bin, by lane, so that fewer wait for one)
-  __shared__ uint32_t part[kWaves], found[2], zeros;
+  __shared__ uint32_t part[kWaves], found[3], zeros;
   __shared__ uint64_t part64[kWaves];
   __shared__ uint16_t order[HELD ? HELD * kThreads : 1u];
   const CacheView& c = a.from;
@@ -176,6 +177,7 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
           if (before < need && need <= before + count) {
             found[0] = bin_of(j);
             found[1] = need - before;
+            found[2] = count;
           }
           before += count;
         }
@@ -183,6 +185,7 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
       prefix |= found[0] << shift;
       known |= (size - 1u) << shift;
       need = found[1];
+      if (need == found[2]) break;  // all of the bin are kept: their other digits do not matter
       __syncthreads();
     }
   }
@@ -195,8 +198,8 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
 #pragma unroll
       for (uint32_t j = 0; j < HELD; ++j) {
         if (j % 4u == 0u && j / 4u >= fours) break;
-        safe |= (asked >> j & 1u) != 0u && rank[j] > prefix ? 1u << j : 0u;
-        equal |= (asked >> j & 1u) != 0u && rank[j] == prefix ? 1u << j : 0u;
+        safe |= (asked >> j & 1u) != 0u && (rank[j] & known) > prefix ? 1u << j : 0u;
+        equal |= (asked >> j & 1u) != 0u && (rank[j] & known) == prefix ? 1u << j : 0u;
       }
     const uint64_t own = (uint64_t)__popc(safe) << 32 | __popc(equal);
     const uint64_t before = block_scan(own, part64, total);
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
     const auto kind = [&](uint32_t i, float v) -> uint32_t {  // 2: kept, 1: equal, 0: not
       if (i >= n) return 0u;
       if (i < lo || i >= hi) return 2u;
-      const uint32_t k = rank_of(v);
+      const uint32_t k = rank_of(v) & known;
       return none ? 0u : k > prefix ? 2u : k == prefix ? 1u : 0u;
     };
     const auto all = [&](auto&& visit) {
@@ -304,8 +307,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs a, uint32_t
 hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
   const CacheView& c = a.from;
   const dim3 heads(c.kv_heads, c.sequences);
-  // (4 heads of 4111 slots, selection and move: held in a place of 16,384 15.8 us, of 32,768
-  // 18.1, read in each pass 18.8; 64 heads of 30,000 slots: held 102 us, read 117.)
+  // (4 heads of 4111 slots, selection and move: held in a place of 16,384 14.4 us, of 32,768
+  // 16.5, read in each pass 16.7; 64 heads of 30,000 slots: held 102 us, read 117.)
   if (c.capacity <= 16u * kThreads)
     evict_select<16><<<heads, kThreads, 0, s>>>(a);
   else if (c.capacity <= 32u * kThreads)
