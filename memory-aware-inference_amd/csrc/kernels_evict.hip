@@ -60,6 +60,11 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
   __shared__ uint16_t order[HELD ? HELD * kThreads : 1u];
   const CacheView& c = a.from;
   const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+  const auto clear = [&](uint32_t size) {
+    for (uint32_t i = tid; i < size; i += kThreads) bins[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid == 0u) zeros = 0u;
+  };
+  clear(2048u);  // (while the length is read)
   const size_t head = (size_t)s * c.kv_heads + h;
   const float* w = a.weights + head * a.weights_stride;
   float* to_w = a.to_weights + head * a.to_weights_stride;
@@ -143,8 +148,7 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs a) {
     for (uint32_t digit = 0; digit < 3u; ++digit) {
       const uint32_t shift = digit == 0u ? 21u : digit == 1u ? 10u : 0u;
       const uint32_t size = digit == 2u ? 1024u : 2048u;
-      for (uint32_t i = tid; i < size; i += kThreads) bins[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (tid == 0u) zeros = 0u;
+      if (digit != 0u) clear(size);
       __syncthreads();
       // (slots that nothing ever saw weigh 0, many of them: counted apart, they do not
       // queue for one bin)
