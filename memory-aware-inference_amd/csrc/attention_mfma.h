@@ -141,7 +141,9 @@ struct Shape {
   static constexpr uint32_t kExchangeBytes =
       VS == 1 ? 0 : kBySlots ? kTeams * kTeamTiles * RT * T::kPieces * 64 * 16 : 2 * kHalves;
   static constexpr uint32_t kOutStride = DW * VS + 4;  // words of a row of the join
-  static constexpr uint32_t kOutBytes = kTeams * 16 * kOutStride * 4;
+  // row tiles joined at once
+  static constexpr uint32_t kOutTiles = RT * kTeams * 16 * kOutStride * 4 <= 144 * 1024 ? RT : 1;
+  static constexpr uint32_t kOutBytes = kOutTiles * kTeams * 16 * kOutStride * 4;
   static constexpr uint32_t kTileBytes = kQueryBytes + kExchangeBytes;
   static constexpr uint32_t kShared = kTileBytes > kOutBytes ? kTileBytes : kOutBytes;
 };
@@ -746,35 +748,43 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       }
     }
     float* join = reinterpret_cast<float*>(shared) + (team * 16u + n) * S::kOutStride;
+    constexpr uint32_t kTileWords = S::kTeams * 16u * S::kOutStride;
 #pragma unroll
-    for (uint32_t r = 0; r < RT; ++r) {
-      exchange_barrier();  // (queries and scores, or the last tile's outputs, are no longer read)
-      float top = -INFINITY;
+    for (uint32_t r0 = 0; r0 < RT; r0 += S::kOutTiles) {
+      exchange_barrier();  // (queries and scores, or the last tiles' outputs, are no longer read)
 #pragma unroll
-      for (uint32_t w = 0; w < S::kSets; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
-      if (wave == 0u) {
-        Joined sum_l;
+      for (uint32_t r = r0; r < r0 + S::kOutTiles; ++r) {
+        float top = -INFINITY;
 #pragma unroll
-        for (uint32_t w = 0; w < S::kSets; ++w)
-          sum_l.add(make_float2(row_m[w][r * 16u + n], row_l[w][r * 16u + n]), top);
-        if (j == 0u) row_sum[r * 16u + n] = sum_l.result(top);
+        for (uint32_t w = 0; w < S::kSets; ++w) top = fmaxf(top, row_m[w][r * 16u + n]);
+        if (wave == r % S::kWaves) {
+          Joined sum_l;
+#pragma unroll
+          for (uint32_t w = 0; w < S::kSets; ++w)
+            sum_l.add(make_float2(row_m[w][r * 16u + n], row_l[w][r * 16u + n]), top);
+          if (j == 0u) row_sum[r * 16u + n] = sum_l.result(top);
+        }
+        const float mine = Joined::times(m[r], top);
+#pragma unroll
+        for (uint32_t u = 0; u < S::kPasses; ++u)
+#pragma unroll
+          for (uint32_t w = 0; w < 4; ++w)
+#pragma unroll
+            for (uint32_t d = 0; d < S::kEach; d += 4) {
+              const f32x4* t = &out[r][u * S::kEach + d];
+              *reinterpret_cast<float4*>(
+                  join + (r - r0) * kTileWords +
+                  ((half * S::kPasses + u) * 16u + j * 4u + w) * S::kEach + d) =
+                  make_float4(t[0][w] * mine, t[1][w] * mine, t[2][w] * mine, t[3][w] * mine);
+            }
       }
-      const float mine = Joined::times(m[r], top);
-#pragma unroll
-      for (uint32_t u = 0; u < S::kPasses; ++u)
-#pragma unroll
-        for (uint32_t w = 0; w < 4; ++w)
-#pragma unroll
-          for (uint32_t d = 0; d < S::kEach; d += 4) {
-            const f32x4* t = &out[r][u * S::kEach + d];
-            *reinterpret_cast<float4*>(
-                join + ((half * S::kPasses + u) * 16u + j * 4u + w) * S::kEach + d) =
-                make_float4(t[0][w] * mine, t[1][w] * mine, t[2][w] * mine, t[3][w] * mine);
-          }
       exchange_barrier();
       constexpr uint32_t kRowThreads = kThreads / 16u;
-      const uint32_t jr = tid / kRowThreads, jn = tid % kRowThreads, out_row = row0 + r * 16u + jr;
-      if (out_row < rows) {
+      const uint32_t jr = tid / kRowThreads, jn = tid % kRowThreads;
+#pragma unroll
+      for (uint32_t r = r0; r < r0 + S::kOutTiles; ++r) {
+        const uint32_t out_row = row0 + r * 16u + jr;
+        if (out_row >= rows) continue;
         const float2 st = row_sum[r * 16u + jr];
         const size_t head = (size_t)kv * rows + out_row;
         const size_t part_row = (size_t)(share + seq) * c.kv_heads * rows + head;
@@ -794,7 +804,8 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
             for (uint32_t w = 0; w < S::kTeams; ++w) {
               const float4 y = *reinterpret_cast<const float4*>(
-                  reinterpret_cast<const float*>(shared) + (w * 16u + jr) * S::kOutStride + d);
+                  reinterpret_cast<const float*>(shared) + (r - r0) * kTileWords +
+                  (w * 16u + jr) * S::kOutStride + d);
               v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
             }
             v.x *= times, v.y *= times, v.z *= times, v.w *= times;
