@@ -37,11 +37,11 @@
 // of the shares.
 //
 // Measured, calls back to back over caches that are not in the L2: one token
-// over 131,071 slots of 4 heads of 256 in BF16 104 us for 537 MB, 5.2 TB/s
+// over 131,071 slots of 4 heads of 256 in BF16 101 us for 537 MB, 5.3 TB/s
 // (5.6 in this kernel), bound by memory; one token a sequence of 24 in F32,
-// 427 MB, 105 us with the weights, of which this kernel has 89; eight drafted
+// 427 MB, 104 us with the weights, of which this kernel has 90; eight drafted
 // tokens a sequence of four, 183 MB, 61 us, bound by the arithmetic of a round
-// and by what comes before the first and behind the last (7 and 4 us); one
+// and by what comes before its loads and behind the last (4 us each); one
 // token over 1021 slots of 8 heads of 128, 4.2 MB, 12.4 us: the launch and a
 // chain of dependent reads (lengths, page numbers, rows, other shares' sums).
 #pragma once
@@ -903,7 +903,7 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   // A few shares are joined by the last of them; many, whose join is more than
   // one workgroup's work, by a kernel of their own.  (1021 slots of 8 heads of
   // 128, four shares: 12.9 us inside, 14.8 with the second kernel.  131,071
-  // slots of 4 heads of 256, 64 shares: the second kernel takes 7 of 104 us.)
+  // slots of 4 heads of 256, 64 shares: the second kernel takes 5.5 of 101 us.)
   const size_t counters = (size_t)a.cache.sequences * a.cache.kv_heads * o.tile_groups;
   if (o.shares > kSharesJoinedInside || counters * 4u + 64u > kWorkspaceCounterBytes)
     o.counters = nullptr;

@@ -42,7 +42,7 @@ __device__ __forceinline__ void load_fours(const float* row, size_t base, size_t
 // ---- softmax ------------------------------------------------------------------
 // y = exp((x - m) / T) / l: a workgroup a chunk of a row, once for the chunk's
 // maximum and sum (scratch), once, with the row's from all of them, for y.  288
-// rows of 151,936 logits: 84 us, 31 and 53, for 350 MB read, read again (half
+// rows of 151,936 logits: 85 us, 31 and 53, for 350 MB read, read again (half
 // of it from the caches) and written, 4.2 TB/s of what has to move once; 5 rows
 // 7.5 us, two launches of little more than an empty one.
 
