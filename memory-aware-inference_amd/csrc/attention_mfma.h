@@ -37,10 +37,10 @@
 // of the shares.
 //
 // Measured, calls back to back over caches that are not in the L2: one token
-// over 131,071 slots of 4 heads of 256 in BF16 101 us for 537 MB, 5.3 TB/s
-// (5.6 in this kernel), bound by memory; one token a sequence of 24 in F32,
-// 427 MB, 104 us with the weights, of which this kernel has 90; eight drafted
-// tokens a sequence of four, 183 MB, 61 us, bound by the arithmetic of a round
+// over 131,071 slots of 4 heads of 256 in BF16 95 us for 537 MB, 5.7 TB/s
+// (6.0 in this kernel), bound by memory; one token a sequence of 24 in F32,
+// 427 MB, 102 us with the weights, of which this kernel has 88; eight drafted
+// tokens a sequence of four, 183 MB, 58 us, bound by the arithmetic of a round
 // and by what comes before its loads and behind the last (4 us each); one
 // token over 1021 slots of 8 heads of 128, 4.2 MB, 12.4 us: the launch and a
 // chain of dependent reads (lengths, page numbers, rows, other shares' sums).
@@ -170,7 +170,8 @@ __device__ __forceinline__ void block_work(const Outputs& o, uint32_t& unit, uin
 
 // FAST: heads of DW * VS values on pages of whole sixteens of slots, so that the
 // slots of a score tile lie one after another and addresses are scalars.
-template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT>
+// ONCE: no other workgroup reads the values, which then pass the caches by.
+template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT, bool ONCE>
 __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Outputs o) {
   using S = Shape<T, DW, VS, RT>;
   constexpr uint32_t kThreads = 64 * S::kWaves, kRound = S::kRound;
@@ -315,11 +316,13 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
           uint32_t at = ((half * S::kPasses + u) * 16u + n) * (S::kWords * 4u);
           if (!FAST) at = min(at, row_bytes - S::kWords * 4u);  // (its outputs are not stored)
           if constexpr (S::kWords == 4) {
-            const u32x4 w = *reinterpret_cast<const Words4*>(p + at);
+            const Words4* from = reinterpret_cast<const Words4*>(p + at);
+            const u32x4 w = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
             for (uint32_t x = 0; x < 4; ++x) value[tile][i][u][x] = w[x];
           } else {
-            const Words2 w = *reinterpret_cast<const Words2*>(p + at);
+            const Words2* from = reinterpret_cast<const Words2*>(p + at);
+            const Words2 w = ONCE ? __builtin_nontemporal_load(from) : *from;
             value[tile][i][u][0] = w.x;
             value[tile][i][u][1] = w.y;
           }
@@ -886,11 +889,11 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
   }
 }
 
-template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT>
+template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT, bool ONCE>
 hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   using S = Shape<T, DW, VS, RT>;
   static const hipError_t attr = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(&attention_mfma<T, DW, VS, FAST, RT>),
+      reinterpret_cast<const void*>(&attention_mfma<T, DW, VS, FAST, RT, ONCE>),
       hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::kShared);
   if (attr != hipSuccess) return attr;
   const uint32_t tiles = row_tiles(a.tokens, a.group);
@@ -903,13 +906,13 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   // A few shares are joined by the last of them; many, whose join is more than
   // one workgroup's work, by a kernel of their own.  (1021 slots of 8 heads of
   // 128, four shares: 12.9 us inside, 14.8 with the second kernel.  131,071
-  // slots of 4 heads of 256, 64 shares: the second kernel takes 5.5 of 101 us.)
+  // slots of 4 heads of 256, 64 shares: the second kernel takes 5.5 of 95 us.)
   const size_t counters = (size_t)a.cache.sequences * a.cache.kv_heads * o.tile_groups;
   if (o.shares > kSharesJoinedInside || counters * 4u + 64u > kWorkspaceCounterBytes)
     o.counters = nullptr;
   const uint32_t units = o.shares * a.cache.kv_heads;
   const uint32_t blocks = o.tile_groups == 1u ? units : (units + 7u) / 8u * 8u * o.tile_groups;
-  attention_mfma<T, DW, VS, FAST, RT><<<blocks, 64 * S::kWaves, S::kShared, s>>>(a, o);
+  attention_mfma<T, DW, VS, FAST, RT, ONCE><<<blocks, 64 * S::kWaves, S::kShared, s>>>(a, o);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || o.shares == 1u || o.counters) return e;
   return launch_attention_join(a, o, s);
@@ -922,20 +925,32 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
 // are shared by slots: 48 rows over 44,236 slots of 4 heads 54 us, three tiles
 // at once, where two waves with half of the head each and two tiles at once
 // took 64.
+//
+// Where that is all of the rows, the values' loads are nontemporal (their lines
+// are whole ones; the keys' come in two halves, and measured slower so).  Over
+// caches that other memory's traffic has driven out of the 256 MB cache
+// 131,071 slots of 4 heads of 256 in BF16 take 94.9 us so and 100.7 without, 48
+// rows over 44,236 slots 57.7 and 60.5, 24 sequences in F32 102.3 and 103.6; over
+// one that it still holds (8 x 4000 slots, 131 MB) 31.9 and 30.8.
+template <typename T, uint32_t DW, uint32_t VS, bool FAST, uint32_t RT>
+hipError_t launch_tiles(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
+  if (row_tiles(a.tokens, a.group) <= RT) return launch_mfma<T, DW, VS, FAST, RT, true>(a, o, s);
+  return launch_mfma<T, DW, VS, FAST, RT, false>(a, o, s);
+}
 template <typename T, uint32_t DIM>
 hipError_t launch_rows(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
   const uint32_t tiles = row_tiles(a.tokens, a.group);
   if (tiles == 1u)
-    return launch_mfma<T, (DIM < 128 ? DIM : 128), (DIM + 127) / 128, true, 1>(a, o, s);
+    return launch_mfma<T, (DIM < 128 ? DIM : 128), (DIM + 127) / 128, true, 1, true>(a, o, s);
   constexpr uint32_t kDw = DIM == 256 ? 64 : DIM, kVs = DIM / kDw;
   if constexpr (DIM != 128 || T::kBytes == 4)
-    if (tiles == 3u || tiles > 4u) return launch_mfma<T, kDw, kVs, true, 3>(a, o, s);
-  return launch_mfma<T, kDw, kVs, true, 2>(a, o, s);
+    if (tiles == 3u || tiles > 4u) return launch_tiles<T, kDw, kVs, true, 3>(a, o, s);
+  return launch_tiles<T, kDw, kVs, true, 2>(a, o, s);
 }
 
 // Heads of 64, 128 and 256 on pages of whole sixteens take scalar addresses
-// (131,071 slots of 4 heads of 256 103.8 us, 105.8 on pages of 24; heads of 128
-// alike), and only they leave the registers for several row tiles.  Others take
+// (131,071 slots of 4 heads of 256 100.5 us, 101.3 on pages of 24; heads of 128
+// and F32 alike), and only they leave the registers for several row tiles.  Others take
 // one row tile at a time, in the next larger shape (8 sequences of 4000 slots of
 // 8 heads: 80 values 24.6 us, 96 26.5, 128 30.8).
 template <typename T>
@@ -946,9 +961,9 @@ hipError_t launch_type(const AttentionArgs& a, const Outputs& o, hipStream_t s) 
     if (dim == 128u) return launch_rows<T, 128>(a, o, s);
     if (dim == 256u) return launch_rows<T, 256>(a, o, s);
   }
-  if (dim <= 64u) return launch_mfma<T, 64, 1, false, 1>(a, o, s);
-  if (dim <= 128u) return launch_mfma<T, 128, 1, false, 1>(a, o, s);
-  return launch_mfma<T, 128, 2, false, 1>(a, o, s);
+  if (dim <= 64u) return launch_tiles<T, 64, 1, false, 1>(a, o, s);
+  if (dim <= 128u) return launch_tiles<T, 128, 1, false, 1>(a, o, s);
+  return launch_tiles<T, 128, 2, false, 1>(a, o, s);
 }
 
 }  // namespace attn
