@@ -144,15 +144,16 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs rope, RopeRows 
   }
 }
 
-// grid (sequences * tokens, slices): the slice's share of the token's query,
-// key and value heads
+// grid (rows, slices): the slice's share of the query, key and value heads of row
+// first + blockIdx.x, of sequences * tokens
 template <uint32_t N, typename T>
 __global__ __launch_bounds__(kThreads) void rope_append_kernel(
-    CacheView cache, RopeArgs rope, uint32_t tokens, const uint32_t* __restrict__ counts,
-    const uint32_t* __restrict__ positions, const float* __restrict__ k, size_t k_stride,
-    const float* __restrict__ v, size_t v_stride, RopeRows q, void* ws) {
+    CacheView cache, RopeArgs rope, uint32_t first, uint32_t tokens,
+    const uint32_t* __restrict__ counts, const uint32_t* __restrict__ positions,
+    const float* __restrict__ k, size_t k_stride, const float* __restrict__ v, size_t v_stride,
+    RopeRows q, void* ws) {
   __shared__ float cs[128], sn[128];
-  const uint32_t row = blockIdx.x, seq = row / tokens, t = row - seq * tokens;
+  const uint32_t row = first + blockIdx.x, seq = row / tokens, t = row - seq * tokens;
   if (t >= brought(counts, seq, tokens)) return;
   const uint32_t slot = held(cache, seq) + t;
   uint32_t at = kNone;
@@ -211,17 +212,29 @@ uint32_t slices_for(uint32_t tokens, uint32_t heads) {
   return std::max(1u, std::min(want, heads));
 }
 
+// A launch takes less than 2^32 threads in x, and runs fewer than it was asked
+// for, without an error, from there on: more rows are several.
+constexpr uint32_t kMostRows = 0xffffffffu / kThreads;
+
 }  // namespace
 
 hipError_t launch_rope(const RopeArgs& rope, const RopeRows& rows, uint32_t tokens,
                        uint32_t head_dim, const uint32_t* positions, hipStream_t s) {
   const bool vec = rope_vectors(rope.rotary_dim, head_dim, rope.layout);
-  const dim3 grid(tokens, slices_for(tokens, rows.heads));
-  if (vec)
-    rope_kernel<4><<<grid, kThreads, 0, s>>>(rope, rows, head_dim, positions);
-  else
-    rope_kernel<1><<<grid, kThreads, 0, s>>>(rope, rows, head_dim, positions);
-  return hipGetLastError();
+  for (uint32_t t0 = 0; t0 < tokens; t0 += std::min(kMostRows, tokens - t0)) {
+    const uint32_t n = std::min(kMostRows, tokens - t0);
+    const dim3 grid(n, slices_for(n, rows.heads));
+    RopeRows part = rows;
+    part.x += t0 * rows.token_stride;
+    part.y += t0 * rows.y_token_stride;
+    if (vec)
+      rope_kernel<4><<<grid, kThreads, 0, s>>>(rope, part, head_dim, positions + t0);
+    else
+      rope_kernel<1><<<grid, kThreads, 0, s>>>(rope, part, head_dim, positions + t0);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_rope_append(const CacheView& cache, const RopeArgs* rope, uint32_t tokens,
@@ -233,18 +246,22 @@ hipError_t launch_rope_append(const CacheView& cache, const RopeArgs* rope, uint
   const bool vec = rope_vectors(r.rotary_dim, cache.head_dim, r.layout) && aligned4(cache.keys) &&
                    aligned4(cache.values);
   const uint32_t rows = cache.sequences * tokens;
-  const dim3 grid(rows, slices_for(rows, qr.heads + 2u * cache.kv_heads));
   auto go = [&](auto kernel) {
-    kernel<<<grid, kThreads, 0, s>>>(cache, r, tokens, counts, positions, k, k_stride, v, v_stride,
-                                     qr, ws);
+    for (uint32_t r0 = 0; r0 < rows; r0 += std::min(kMostRows, rows - r0)) {
+      const uint32_t n = std::min(kMostRows, rows - r0);
+      const dim3 grid(n, slices_for(n, qr.heads + 2u * cache.kv_heads));
+      kernel<<<grid, kThreads, 0, s>>>(cache, r, r0, tokens, counts, positions, k, k_stride, v,
+                                       v_stride, qr, ws);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
   };
   if (cache.type == kKvF32)
-    vec ? go(rope_append_kernel<4, float>) : go(rope_append_kernel<1, float>);
-  else if (cache.type == kKvF16)
-    vec ? go(rope_append_kernel<4, __half>) : go(rope_append_kernel<1, __half>);
-  else
-    vec ? go(rope_append_kernel<4, __hip_bfloat16>) : go(rope_append_kernel<1, __hip_bfloat16>);
-  return hipGetLastError();
+    return vec ? go(rope_append_kernel<4, float>) : go(rope_append_kernel<1, float>);
+  if (cache.type == kKvF16)
+    return vec ? go(rope_append_kernel<4, __half>) : go(rope_append_kernel<1, __half>);
+  return vec ? go(rope_append_kernel<4, __hip_bfloat16>) : go(rope_append_kernel<1, __hip_bfloat16>);
 }
 
 hipError_t launch_kv_advance(const CacheView& cache, const uint32_t* counts, uint32_t more,

@@ -199,3 +199,35 @@ def test_rows_beyond_four_gigabytes(hip_ctx, dev):
                                   R.to_bf16(k[t, head]))
             assert np.array_equal(dev.ctx.from_device(values + at, (dim,), np.uint16),
                                   R.to_bf16(v[t, head]))
+
+
+def test_more_tokens_than_a_launch_has_threads_for(hip_ctx, dev):
+    """2^24 tokens and some: a workgroup of 256 threads each is 2^32 threads."""
+    n = (1 << 24) + 5
+    rng = np.random.default_rng(6)
+    rope, inv, mag = make_rope(dev, 2, 1e4)
+    x = rng.standard_normal((n, 2)).astype(np.float32)
+    pos = np.arange(n, dtype=np.uint32)
+    d_x, d_p = dev.put(x), dev.put(pos)
+    d_y = dev.put(np.full_like(x, 7.0))
+    hip_ctx.rope_device(rope, d_x, n, 1, 2, d_p, d_y)
+    hip_ctx.synchronize()
+    want, size = R.rotate(x[:, None], pos, inv, mag, 0)
+    # beyond 2^20 positions the f64 reference's angle is itself off by pos * 2^-53 radians
+    check(dev.get(d_y, x)[:, None], want, size + 1e-8)
+
+    page = 1 << 12
+    pages = n // page + 1
+    order = rng.permutation(pages).astype(np.uint32)
+    d_keys, d_values = (dev.put(np.full((pages * page, 2), 3.0, np.float32)) for _ in range(2))
+    h = si_hip.KvCache(ggml_type=0, kv_heads=1, head_dim=2, page_tokens=page, pages=pages,
+                       sequences=1, max_pages=pages, d_keys=d_keys, d_values=d_values,
+                       d_page_table=dev.put(order), d_lengths=dev.put(np.zeros(1, np.uint32)))
+    hip_ctx.rope_append_device(h, n, d_x, d_x, rope=rope, d_q=d_x, heads=1, d_q_out=d_y)
+    hip_ctx.synchronize()
+    check(dev.get(d_y, x)[:, None], want, size + 1e-8, "query")
+    slots = np.arange(n)
+    row = order[slots // page].astype(np.int64) * page + slots % page
+    like = np.empty((pages * page, 2), np.float32)
+    assert np.array_equal(dev.get(d_values, like)[row], x)
+    check(dev.get(d_keys, like)[row][:, None], want, size + 1e-8, "keys")
