@@ -112,8 +112,8 @@ __global__ __launch_bounds__(kThreads) void attention_generic(AttentionArgs a, f
 }
 
 // weights[slot] += sum over the kv head's rows of exp2(score - m) / l.  grid
-// (slots / (256 / PARTS), kv_heads, sequences): the waves of a workgroup add up
-// 1 / PARTS of the rows each, in their order, kAhead rows' loads under way at
+// (blocks of 256 / PARTS slots, from `first_block` on, kv_heads, sequences): the waves
+// of a workgroup add up 1 / PARTS of the rows each, in their order, kAhead rows' loads under way at
 // once; the parts are added in theirs.  Up to eight rows are one part, more
 // four (24 sequences of 2000 slots, four rows a head: with the attention 96.4
 // us in one part, 106.3 in four; 25 of 65 slots, 112 rows: 47.9 and 39.1, 72.1
@@ -122,16 +122,18 @@ constexpr uint32_t kFewRows = 8;
 template <uint32_t PARTS>
 __global__ __launch_bounds__(kThreads) void attention_weights(AttentionArgs a, const float2* stats,
                                                               const float* scores,
-                                                              uint32_t score_stride) {
+                                                              uint32_t score_stride,
+                                                              uint32_t first_block) {
   constexpr uint32_t kSlots = kThreads / PARTS, kAhead = PARTS == 1 ? 4 : 8;
   __shared__ float sums[PARTS][kSlots];
   const CacheView& c = a.cache;
   const uint32_t lane = threadIdx.x % kSlots, part = uniform(threadIdx.x / kSlots);
-  const uint32_t slot = blockIdx.x * kSlots + lane, kv = blockIdx.y, s = blockIdx.z;
+  const uint32_t slot0 = (first_block + blockIdx.x) * kSlots, slot = slot0 + lane;
+  const uint32_t kv = blockIdx.y, s = blockIdx.z;
   const uint32_t count = brought(a.counts, s, a.tokens), length = held(c, s);
   const uint32_t rows = a.tokens * a.group, used = count * a.group;
   const uint32_t slots = min(length + count, c.capacity);
-  if (count == 0u || blockIdx.x * kSlots >= slots) return;
+  if (count == 0u || slot0 >= slots) return;
   const size_t at = ((size_t)s * c.kv_heads + kv) * rows;
   const uint32_t each = (used + PARTS - 1u) / PARTS;
   const uint32_t first = min(part * each, used), last = min(first + each, used);
@@ -170,6 +172,24 @@ __global__ __launch_bounds__(kThreads) void attention_weights(AttentionArgs a, c
   a.weights[((size_t)s * c.kv_heads + kv) * a.weights_stride + slot] += sum;
 }
 
+// (A launch takes less than 2^32 threads in x, and runs fewer than it was asked for, without an
+// error, from there on.)
+template <uint32_t PARTS>
+hipError_t launch_weights(const AttentionArgs& a, const float2* stats, const float* scores,
+                          uint32_t score_stride, hipStream_t s) {
+  constexpr uint32_t kSlots = kThreads / PARTS, kMost = 0xffffffffu / kThreads;
+  const CacheView& c = a.cache;
+  const uint32_t blocks = (c.capacity + kSlots - 1u) / kSlots;
+  for (uint32_t b = 0; b < blocks; b += std::min(kMost, blocks - b)) {
+    attention_weights<PARTS>
+        <<<dim3(std::min(kMost, blocks - b), c.kv_heads, c.sequences), kThreads, 0, s>>>(
+            a, stats, scores, score_stride, b);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 }  // namespace
 
 size_t attention_workspace_bytes(const CacheView& cache, uint32_t heads, uint32_t tokens,
@@ -199,13 +219,8 @@ hipError_t launch_attention(const AttentionArgs& a, bool tuned, hipStream_t s) {
     e = hipGetLastError();
   }
   if (e != hipSuccess || !a.weights) return e;
-  if (a.tokens * a.group <= kFewRows)
-    attention_weights<1><<<dim3((c.capacity + 255u) / 256u, c.kv_heads, c.sequences), kThreads, 0,
-                           s>>>(a, stats, scores, sp.score_stride);
-  else
-    attention_weights<4><<<dim3((c.capacity + 63u) / 64u, c.kv_heads, c.sequences), kThreads, 0,
-                           s>>>(a, stats, scores, sp.score_stride);
-  return hipGetLastError();
+  if (a.tokens * a.group <= kFewRows) return launch_weights<1>(a, stats, scores, sp.score_stride, s);
+  return launch_weights<4>(a, stats, scores, sp.score_stride, s);
 }
 
 }  // namespace sihip

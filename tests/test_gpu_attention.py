@@ -321,3 +321,28 @@ def test_captured_steps(hip_ctx, dev):
         check(dev.get(d_w, weights), total, total_tol, f"weights {step}")
         c.lengths = c.lengths + 1
         assert np.array_equal(dev.get(c.d_lengths, c.lengths), c.lengths)
+
+
+def test_weights_of_a_capacity_beyond_one_launch(hip_ctx, dev):
+    """Weights of a table of 2^30 slots, few of them in use: four workgroups of 64 threads each
+    for 64 slots are more threads than a launch takes."""
+    rng = np.random.default_rng(17)
+    c = R.Cache(dev, rng, "f16", 1, 1, 64, 16, 20, [300])
+    tokens, heads = 5, 2
+    q = rng.standard_normal((1, tokens, heads, 64)).astype(np.float32)
+    want, tol, w, wtol = R.attention(c, q, 0.125, 0, None)
+    c.handle.max_pages = (1 << 26) + 1
+    table = dev.raw(4 * c.handle.max_pages)
+    dev.ctx.to_device(table, c.table)
+    c.handle.d_page_table = table
+    capacity = c.handle.capacity
+    d_w = dev.raw(4 * capacity)
+    old = rng.random((1, 1, c.capacity)).astype(np.float32)
+    dev.ctx.to_device(d_w, old)
+    size = hip_ctx.paged_attention_workspace(c.handle, heads, tokens, True)
+    d_out = dev.put(np.full(q.shape, 9.0, np.float32))
+    hip_ctx.paged_attention_device(c.handle, heads, tokens, 0.125, dev.put(q), d_out, dev.raw(size),
+                                   size, d_weights=d_w, weights_stride=capacity)
+    hip_ctx.synchronize()
+    check(dev.get(d_out, q), want, tol)
+    check(dev.get(d_w, old), old + w, wtol + 2.0 ** -23 * (old + w))
