@@ -136,6 +136,10 @@ int si_hip_kv_advance_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
  * is zeros.  Slots that a row does not see have no part in it, whatever they
  * hold: NaN and infinities in them do not reach it.  A row that sees a key or
  * value that is no finite number is not a number, in part or as a whole.
+ * Sums, maxima and exponentials are f32.  Over an F16 cache a row's query values
+ * are held to 22 bits down to 2^-28 of the largest and smaller ones to 2^-51 of it,
+ * its p_i to 22 bits down to 2^-17 of the largest and smaller ones to 2^-39 of it;
+ * over the others both to 24 bits.
  *
  * With d_weights, [sequences][kv_heads][weights_stride], entry i of kv head h
  * grows by the sum of p_i over the head's query heads and the new tokens;

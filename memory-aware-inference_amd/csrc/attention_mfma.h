@@ -16,10 +16,14 @@
 //
 // Precision: q and p are f32.  With a 16-bit cache they go to the matrix cores
 // as sums of 16-bit numbers: for BF16 three, the leading 8 bits, the next 8
-// and the last 8 (exact); for F16 two of 11 bits, q scaled by a power of two
-// that puts its row's largest value at 2^14, and p times 2^14, so that neither
-// half loses bits to F16's range.  An f32 cache takes the f32 instructions.
-// Products and sums are f32.
+// and the last 8 (exact); for F16 two of 11 bits, 22 of the 24, for a third
+// would cost half as many products again.  F16's least step, 2^-24, sets how far
+// these reach: q is scaled by a power of two that puts its row's largest value at
+// 2^14, and its second piece, whose sum is one of its own, by 2^12 more, so that
+// values down to 2^-28 of the largest have their 22 bits, and smaller ones are
+// good to 2^-51 of it; p is taken times 2^14, both pieces, for they share their sum:
+// 22 bits down to 2^-17, and smaller ones good to 2^-39 of the row's largest.  An
+// f32 cache takes the f32 instructions.  Products and sums are f32.
 //
 // A wave has up to 128 values of a head.  Larger heads are a team's.  For one
 // row tile two waves take a half each, of the keys and of the values: they add
@@ -66,12 +70,14 @@ struct Bf16 {
   // (words of values: exponents, and what carries out of one that is all ones)
   static constexpr uint32_t kSlots = 32, kBytes = 2, kPieces = 3;
   static constexpr float kShift = 0.0f;  // p is held times 2^kShift
+  static constexpr float kQueryRest = 1.0f;  // what a query's last piece is held times
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   // The pieces of x and y, in the halves of one word each.  What is no number
   // is its first piece alone.
+  template <bool QUERY>
   static __device__ __forceinline__ void split(float x, float y, uint32_t (&w)[kPieces]) {
     const uint32_t top = 0xffff0000u;
     float r = x, s = y;
@@ -89,13 +95,16 @@ struct Bf16 {
 struct F16 {
   static constexpr uint32_t kSlots = 32, kBytes = 2, kPieces = 2;
   static constexpr float kShift = 14.0f;
+  static constexpr float kQueryRest = 0x1p12f;  // (a rest of at most 2^3)
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
+  template <bool QUERY>
   static __device__ __forceinline__ void split(float x, float y, uint32_t (&w)[kPieces]) {
+    const float rest = QUERY ? kQueryRest : 1.0f;
     const _Float16 a = (_Float16)x, b = (_Float16)y;
-    const _Float16 c = (_Float16)(x - (float)a), d = (_Float16)(y - (float)b);
+    const _Float16 c = (_Float16)((x - (float)a) * rest), d = (_Float16)((y - (float)b) * rest);
     w[0] = (uint32_t)__builtin_bit_cast(uint16_t, a) |
            (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
     w[1] = (uint32_t)__builtin_bit_cast(uint16_t, c) |
@@ -106,7 +115,7 @@ struct F16 {
 };
 struct F32 {
   static constexpr uint32_t kSlots = 16, kBytes = 4, kPieces = 1;
-  static constexpr float kShift = 0.0f;
+  static constexpr float kShift = 0.0f, kQueryRest = 1.0f;
   static constexpr uint32_t kExponent = 0x7f800000u, kUnit = 0x00800000u, kCarry = 0x80000000u;
 };
 
@@ -406,7 +415,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
         for (uint32_t v = 0; v < 8; v += 2) {
           uint32_t p[T::kPieces];
-          T::split(x[k][v] * s, x[k][v + 1] * s, p);
+          T::template split<true>(x[k][v] * s, x[k][v + 1] * s, p);
 #pragma unroll
           for (uint32_t q = 0; q < T::kPieces; ++q) w[q][v / 2] = p[q];
         }
@@ -495,7 +504,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
         for (uint32_t i = 0; i < S::kOwnRows; i += 2) {
           uint32_t w[T::kPieces];
-          T::split(p[i], p[i + 1], w);
+          T::template split<false>(p[i], p[i + 1], w);
 #pragma unroll
           for (uint32_t k = 0; k < T::kPieces; ++k) b[k][i / 2] = w[k];
         }
@@ -606,6 +615,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
 #pragma unroll
         for (uint32_t s = 0; s < S::kOwnSubs; ++s) {
           sum[r][s] = piece[s][kSums - 1];
+          if (T::kQueryRest != 1.0f) sum[r][s] *= 1.0f / T::kQueryRest;
 #pragma unroll
           for (int k = (int)kSums - 2; k >= 0; --k) sum[r][s] += piece[s][k];
           if (T::kShift != 0.0f) sum[r][s] *= unscale[r];

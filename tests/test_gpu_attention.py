@@ -346,3 +346,47 @@ def test_weights_of_a_capacity_beyond_one_launch(hip_ctx, dev):
     hip_ctx.synchronize()
     check(dev.get(d_out, q), want, tol)
     check(dev.get(d_w, old), old + w, wtol + 2.0 ** -23 * (old + w))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,dim", [(4, 128), (20, 128), (4, 256), (20, 256), (4, 80)])
+def test_one_query_value_far_above_the_others(hip_ctx, dev, kind, heads, dim):
+    """Where the keys are zero beside it, the others alone make the scores.  They lie down to
+    2^-28 of it, where an F16 cache's calls hold 22 bits of them: 2 units in the last place
+    of sum |q k| at most, within the 16 of the tolerance."""
+    rng = np.random.default_rng(heads + dim)
+    c = R.Cache(dev, rng, kind, 3, 2, dim, 16, 14, [200, 33, 7])
+    c.keys[..., 0] = 0
+    c.keys[..., dim - 1] = 0
+    c.upload()
+    q = rng.uniform(1.0, 2.0, (3, 2, heads, dim)) * rng.choice([-1.0, 1.0], (3, 2, heads, dim))
+    q[:, 0, :, 0] = 2.0 ** 28
+    q[:, 1, :, dim - 1] = -2.0 ** 20
+    run(hip_ctx, dev, c, q.astype(np.float32), weights=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,dim", [(4, 128), (20, 128), (20, 256), (4, 80)])
+@pytest.mark.parametrize("bits", [12, 24, 34])
+def test_weights_far_below_the_largest(hip_ctx, dev, kind, heads, dim, bits):
+    """A first slot that outweighs each other one 2^bits times, with values of 0: the others
+    alone make the output.  An F16 cache's calls hold their p to 2^-39 of the largest."""
+    rng = np.random.default_rng(heads + dim + bits)
+    c = R.Cache(dev, rng, kind, 3, 2, dim, 16, 14, [200, 33, 7])
+    scale = float(np.float32(dim ** -0.5))
+    c.keys = R.encode(R.decode(c.keys, kind) * 0.1, kind)
+    for s in range(3):
+        p, o = c.at(s, 0)
+        c.keys[p, :, o] = R.encode(np.full(dim, bits * np.log(2.0) / (scale * dim)), kind)
+        c.values[p, :, o] = 0
+    c.upload()
+    q = rng.uniform(0.98, 1.02, (3, 2, heads, dim)).astype(np.float32)
+    want, tol, _, _ = R.attention(c, q, scale, 0, None)
+    assert np.all(np.abs(want) < 200 * 8 * 2.0 ** -(0.9 * bits))
+    if kind == "f16":
+        for s, n in enumerate(c.lengths):
+            for kv in range(2):
+                v = np.abs(c.rows("values", s, kv, np.arange(int(n) + 2))).sum(0)
+                tol[s, :, kv * heads // 2:(kv + 1) * heads // 2] += 2.0 ** -39 * v
+    for policy in both_policies(hip_ctx):
+        check(attend(hip_ctx, dev, c, q, scale), want, tol, policy)
