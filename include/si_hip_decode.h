@@ -134,7 +134,8 @@ int si_hip_kv_advance_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
  * q_head_stride; d_out contiguous [sequences][tokens][heads][head_dim].  A row
  * with nothing to attend to (t >= d_counts[s], slots on pages beyond the pool)
  * is zeros.  Slots that a row does not see have no part in it, whatever they
- * hold: NaN and infinities in them do not reach it.  A row that sees a key or
+ * hold: NaN and infinities in them do not reach it, and a page before the window
+ * may lie beyond the pool.  A row that sees a key or
  * value that is no finite number is not a number, in part or as a whole.
  * Sums, maxima and exponentials are f32.  Over an F16 cache a row's query values
  * are held to 22 bits down to 2^-28 of the largest and smaller ones to 2^-51 of it,

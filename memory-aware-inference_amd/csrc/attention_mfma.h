@@ -240,7 +240,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
       uint32_t at[kPlaces];
     };
     const uint32_t* table = c.table + (size_t)seq * c.max_pages;
-    uint32_t bad = 0u;
+    uint32_t bad = 0u;  // the end of the last slots whose page lies beyond the pool
     const auto pages_of = [&](uint32_t base) {
       Place p;
       if constexpr (FAST) {
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
             p.at[s] = (page.at[s] * c.kv_heads + kv) * c.page_tokens +
                       (slot - divided(slot, c.div_mul, c.div_shift) * c.page_tokens);
           else
-            bad = 1u;
+            bad = slot + (FAST ? 16u : 1u);
         }
       }
       return p;
@@ -743,7 +743,8 @@ __global__ __launch_bounds__(512, 2) void attention_mfma(AttentionArgs a, Output
         load_values(row, 0u);  // the next tile's
       }
     }
-    if (bad) report_device_error(a.report, kDevErrCachePage);
+    // (slots before the window need no page)
+    if (bad > any_lo) report_device_error(a.report, kDevErrCachePage);
 
     // ---- the waves join
     // A row with slots whose scores are all -inf (0 / 0 in the end) has l = -1

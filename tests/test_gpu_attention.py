@@ -390,3 +390,32 @@ def test_weights_far_below_the_largest(hip_ctx, dev, kind, heads, dim, bits):
                 tol[s, :, kv * heads // 2:(kv + 1) * heads // 2] += 2.0 ** -39 * v
     for policy in both_policies(hip_ctx):
         check(attend(hip_ctx, dev, c, q, scale), want, tol, policy)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page", [1, 8, 16, 24, 32])
+@pytest.mark.parametrize("heads,dim,tokens", [(4, 64, 1), (20, 128, 3), (12, 256, 5), (6, 80, 3)])
+def test_pages_behind_the_window(hip_ctx, dev, kind, page, heads, dim, tokens):
+    """A page that no row sees any more may lie anywhere; one with a seen slot is reported."""
+    window = 40
+    rng = np.random.default_rng(page * 1000 + dim)
+    c = R.Cache(dev, rng, kind, 4, 2, dim, page, -(-320 // page), [100, 61, 300, 12])
+    for s, n in enumerate(c.lengths):
+        c.table[s, :max(0, int(n) + 1 - window) // page] = 0xFFFFFFFF
+    assert (c.table[0, 0] == 0xFFFFFFFF) and c.table[3, 0] != 0xFFFFFFFF
+    c.upload()
+    q = rng.standard_normal((4, tokens, heads, dim)).astype(np.float32)
+    run(hip_ctx, dev, c, q, window=window, weights=True)
+    c.table[2, (301 - window) // page] = 0xFFFFFFFF  # the one with the first slot that is seen
+    c.upload()
+    scale = float(np.float32(dim ** -0.5))
+    want, tol, _, _ = R.attention(c, q, scale, window, None)
+    for policy in both_policies(hip_ctx):
+        size = hip_ctx.paged_attention_workspace(c.handle, heads, tokens)
+        d_out = dev.put(np.full(q.shape, 9.0, np.float32))
+        hip_ctx.paged_attention_device(c.handle, heads, tokens, scale, dev.put(q), d_out,
+                                       dev.raw(size), size, window=window)
+        with pytest.raises(HipError) as e:
+            hip_ctx.synchronize()
+        assert "pool" in e.value.message
+        check(dev.get(d_out, q), want, tol, policy)
