@@ -88,7 +88,7 @@ typedef struct si_hip_rope {
  * pair that turns t times within original_length positions, the frequencies
  * go from unchanged at floor(dim(beta_fast)) to divided by factor at
  * ceil(dim(beta_slow)) along a linear ramp, and *magnitude is
- * 0.1 ln(factor) + 1 (1 without it).  factor, original_length and the betas
+ * 0.1 ln(factor) + 1 where factor > 1 (1 else, and without YARN).  factor, original_length and the betas
  * are read where the scaling uses them. */
 int si_hip_rope_frequencies(size_t rotary_dim, double theta, uint32_t scaling, double factor,
                             double original_length, double beta_fast, double beta_slow,

@@ -148,7 +148,7 @@ int si_hip_rope_frequencies(size_t rotary_dim, double theta, uint32_t scaling, d
     const long double fixed = std::rint(turns * 18446744073709551616.0L);
     frequencies[i] = fixed >= 18446744073709551616.0L ? 0u : (uint64_t)fixed;
   }
-  *magnitude = yarn ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+  *magnitude = yarn && factor > 1.0 ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
   return clear_error();
 }
 

@@ -168,3 +168,11 @@ def test_rope_frequencies_refusals():
     assert call(sc=1, fa=0.0) == DIM and call(sc=1, fa=float("inf")) == DIM
     assert call(sc=2, th=1.0) == DIM and call(sc=2, ol=0.0) == DIM and call(sc=2, bs=0.0) == DIM
     assert call(sc=2, bf=0.5) == DIM and call(tab=None) == NULL
+
+
+def test_yarn_magnitude_of_a_factor_below_one():
+    """The logarithm's growth is of stretched contexts; others keep their magnitude."""
+    for factor, want in [(1e-6, 1.0), (0.5, 1.0), (1.0, 1.0), (1.5, 0.1 * np.log(1.5) + 1.0),
+                         (40.0, 0.1 * np.log(40.0) + 1.0)]:
+        _, magnitude = si_hip.rope_frequencies(64, 1e4, si_hip.ROPE_SCALING_YARN, factor, 32768.0)
+        assert magnitude == pytest.approx(want, rel=1e-7)
