@@ -73,7 +73,8 @@ typedef struct si_hip_kv_cache {
  * turns by p * d_frequencies[i] / 2^64 of a full turn, (a, b) -> magnitude *
  * (a cos - b sin, b cos + a sin).  As fractions of a turn in 64-bit fixed
  * point the product's whole turns drop out in the wrapping multiplication, so
- * the angle is exact to 2^-32 of a turn at position 2^32 - 1. */
+ * an entry's own error, times the position, is the angle's: half a unit of
+ * 2^-64 of a turn makes 2^-33 at position 2^32 - 1. */
 typedef struct si_hip_rope {
   uint32_t layout;
   uint32_t rotary_dim; /* even, at least 2 */
@@ -88,8 +89,9 @@ typedef struct si_hip_rope {
  * pair that turns t times within original_length positions, the frequencies
  * go from unchanged at floor(dim(beta_fast)) to divided by factor at
  * ceil(dim(beta_slow)) along a linear ramp, and *magnitude is
- * 0.1 ln(factor) + 1 where factor > 1 (1 else, and without YARN).  factor, original_length and the betas
- * are read where the scaling uses them. */
+ * 0.1 ln(factor) + 1 where factor > 1 (1 else, and without YARN).  factor,
+ * original_length and the betas are read where the scaling uses them.  Entries
+ * are good to two units of 2^-64 of a turn where factor >= 1. */
 int si_hip_rope_frequencies(size_t rotary_dim, double theta, uint32_t scaling, double factor,
                             double original_length, double beta_fast, double beta_slow,
                             uint64_t *frequencies, float *magnitude);

@@ -124,26 +124,29 @@ int si_hip_rope_frequencies(size_t rotary_dim, double theta, uint32_t scaling, d
                  beta_fast >= beta_slow)))
     return set_error(SI_HIP_ERR_DIMENSIONS, "rotary scaling parameters are invalid");
   if (!frequencies || !magnitude) return set_error(SI_HIP_ERR_NULL, "rotary frequencies are null");
-  const double n = (double)rotary_dim, pi = 3.14159265358979323846;
-  double low = 0.0, high = 0.0;
+  // (Arithmetic of 64 bits, for 64-bit entries: with one of 53 the angle 2^32 positions on would
+  // be off by up to 2^-25 of a turn.)
+  const long double n = (long double)rotary_dim, pi = 3.14159265358979323846264338327950288L;
+  long double low = 0.0L, high = 0.0L;
   if (yarn) {
-    auto dim = [&](double turns) {
-      return n * std::log(original_length / (2.0 * pi * turns)) / (2.0 * std::log(theta));
+    auto dim = [&](long double turns) {
+      return n * std::log(original_length / (2.0L * pi * turns)) /
+             (2.0L * std::log((long double)theta));
     };
-    low = std::fmax(std::floor(dim(beta_fast)), 0.0);
-    high = std::fmin(std::ceil(dim(beta_slow)), n - 1.0);
+    low = std::fmax(std::floor(dim(beta_fast)), 0.0L);
+    high = std::fmin(std::ceil(dim(beta_slow)), n - 1.0L);
   }
   for (size_t i = 0; i < rotary_dim / 2; ++i) {
-    double f = std::pow(theta, -2.0 * (double)i / n);
+    long double f = std::pow((long double)theta, -2.0L * (long double)i / n);
     if (scaling == SI_HIP_ROPE_SCALING_LINEAR) {
       f /= factor;
     } else if (yarn) {
-      const double at = ((double)i - low) / std::fmax(high - low, 0.001);
-      const double ramp = std::fmin(std::fmax(at, 0.0), 1.0);
-      f = f / factor * ramp + f * (1.0 - ramp);
+      const long double at = ((long double)i - low) / std::fmax(high - low, 0.001L);
+      const long double ramp = std::fmin(std::fmax(at, 0.0L), 1.0L);
+      f = f / factor * ramp + f * (1.0L - ramp);
     }
     // the fraction of a turn: whole turns a position (factor < 1) change no angle
-    long double turns = (long double)f / (2.0L * 3.14159265358979323846264338327950288L);
+    long double turns = f / (2.0L * pi);
     turns -= std::floor(turns);
     const long double fixed = std::rint(turns * 18446744073709551616.0L);
     frequencies[i] = fixed >= 18446744073709551616.0L ? 0u : (uint64_t)fixed;

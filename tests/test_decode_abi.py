@@ -176,3 +176,30 @@ def test_yarn_magnitude_of_a_factor_below_one():
                          (40.0, 0.1 * np.log(40.0) + 1.0)]:
         _, magnitude = si_hip.rope_frequencies(64, 1e4, si_hip.ROPE_SCALING_YARN, factor, 32768.0)
         assert magnitude == pytest.approx(want, rel=1e-7)
+
+
+@pytest.mark.parametrize("n,theta,scaling,factor", [
+    (64, 1e7, 0, 1.0), (128, 1e6, 0, 1.0), (256, 12345.678, 0, 1.0), (128, 1e6, 1, 3.7),
+    (128, 1e6, 2, 4.0), (256, 5e5, 2, 7.3), (64, 1e4, 2, 0.9)])
+def test_rope_frequencies_to_the_last_bits(n, theta, scaling, factor):
+    """Entries against 60 digits.  In arithmetic of 64 bits a frequency of at most a radian, 0.16
+    turns, is off by some ten roundings of 2^-64, less than a unit of 2^-64 turns in all, and the
+    entry's own rounding is half of one: so at most two, 2^-31 of a turn at the last position."""
+    from decimal import ROUND_CEILING, ROUND_FLOOR, Decimal, localcontext
+    table, _ = si_hip.rope_frequencies(n, theta, scaling, factor, 32768.0)
+    with localcontext() as c:
+        c.prec = 60
+        pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+        log_theta, f = Decimal(theta).ln(), Decimal(factor)
+        dim = lambda t: n * (Decimal(32768) / (2 * pi * t)).ln() / (2 * log_theta)  # noqa: E731
+        low = max(dim(32).to_integral_value(ROUND_FLOOR), Decimal(0))
+        high = min(dim(1).to_integral_value(ROUND_CEILING), Decimal(n - 1))
+        for i in range(n // 2):
+            inv = (-2 * Decimal(i) / n * log_theta).exp()
+            if scaling == 1:
+                inv /= f
+            elif scaling == 2:
+                ramp = min(max((i - low) / max(high - low, Decimal("0.001")), Decimal(0)), Decimal(1))
+                inv = inv / f * ramp + inv * (1 - ramp)
+            exact = inv / (2 * pi) * Decimal(2) ** 64
+            assert abs(Decimal(int(table[i])) - exact) <= 2, i
