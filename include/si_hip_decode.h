@@ -192,9 +192,10 @@ int si_hip_softmax_device(si_hip_context *ctx, const float *d_x, size_t rows, si
  * Draft i, token x, is accepted while u_i q_i(x) < p_i(x).  After the first
  * that is not, the next token is drawn from max(p_i - q_i, 0), or, where that
  * is zero throughout or all drafts were accepted, from p: the lowest token whose
- * running sum exceeds u_drafts times the whole sum.  Each term is clamped to
- * [0, 1] (a NaN counts as 0) and taken down to a multiple of 2^-36, so the sums
- * are exact in any order and so is the token.
+ * running sum exceeds u_drafts, taken down to a multiple of 2^-24, times the
+ * whole sum.  Each term is clamped to [0, 1] (a NaN counts as 0) and taken down
+ * to a multiple of 2^-36, so the sums (below 2^28) are exact in any order and so
+ * is the token.
  * d_accepted[s]: the number accepted; d_out_tokens [sequences][drafts + 1]:
  * those tokens, the drawn one, then SI_HIP_TOKEN_NONE.  A drafted token beyond
  * the vocabulary is refused and reported; so is a row of probabilities that is

@@ -325,6 +325,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, uint64_t
     __syncthreads();
     add_chunks();
   }
+  // (u in steps of 2^-24, those that a float has just below 1: the product is an integer's)
   const float u = a.uniform[(size_t)s * (a.drafts + 1u) + a.drafts];
   const uint32_t n24 = u > 0.0f ? (uint32_t)fminf(u * 0x1p24f, 16777215.0f) : 0u;
   const uint64_t threshold = __umul64hi(total, n24) << 40 | (total * n24) >> 24;

@@ -235,3 +235,20 @@ def test_verify_in_a_graph(hip_ctx, dev):
         want_a, want_o = R.verify(p.reshape(n, m + 1, vocab), None, tokens, None, uniform, vocab)
         assert np.array_equal(dev.get(d_a, np.empty(n, np.uint32)), want_a)
         assert np.array_equal(dev.get(d_o, np.empty((n, m + 1), np.uint32)), want_o)
+
+
+def test_draw_in_steps_of_a_uniform_number(hip_ctx, dev):
+    """The number that draws is taken down to a multiple of 2^-24: below that the first token with
+    any mass is drawn, though the numbers themselves lie beyond it."""
+    vocab = 6000
+    target = np.zeros((6, 2, vocab), np.float32)
+    target[:, :, 17] = 2.0 ** -30
+    target[:, :, 4100] = 2.0 ** -24
+    target[:, :, 5000] = 1.0 - 2.0 ** -23
+    tokens = np.zeros((6, 1), np.uint32)
+    uniform = np.zeros((6, 2), np.float32)
+    uniform[:, 1] = [0.0, 2.0 ** -29, 2.0 ** -24 - 2.0 ** -48, 2.0 ** -24, 1.5 * 2.0 ** -24, 2.0 ** -23]
+    accepted, out, error = check(hip_ctx, dev, target, None, tokens, np.zeros(6, np.uint32), uniform,
+                                 vocab)
+    assert error is None and not accepted.any()
+    assert out[:, 0].tolist() == [17, 17, 17, 4100, 4100, 5000]
