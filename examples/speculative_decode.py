@@ -146,7 +146,12 @@ class SpeculativeDecoder:
         kv = self.kv_heads * self.head_dim
         cache = self.caches[which]
         norm = lambda x, y: self._call(lib.si_hip_rms_norm_device, 1, x, None, self.norm, n, h, 1e-6, y)  # noqa: E731
-        times = lambda w, rows, x, y: self._call(lib.si_hip_matmul_many_device, w.handle, rows, h, n, x, y)  # noqa: E731
+
+        def times(w, rows, x, y):  # (a product takes up to MAX_BATCH rows of x)
+            for r in range(0, n, si_hip.MAX_BATCH):
+                self._call(lib.si_hip_matmul_many_device, w.handle, rows, h,
+                           min(n - r, si_hip.MAX_BATCH), x + 4 * r * h, y + 4 * r * rows)
+
         self._call(lib.si_hip_embedding_device, self.embed.handle, h, self.vocab, self.d_ids, n, self.d_x)
         norm(self.d_x, self.d_h)
         times(self.w_q, h, self.d_h, self.d_q)

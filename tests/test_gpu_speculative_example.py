@@ -87,3 +87,27 @@ def test_every_step(hip_ctx, kind):
     assert d.evictions >= 1
     for x in decoders:
         x.close()
+
+
+def test_more_rows_than_one_product_takes(hip_ctx):
+    """Five sequences of four rows: products of sixteen rows and of four.  A row's logits are its
+    own: both are far closer than 2^-15 of |w| |h| to the product, another row's lie about |w| |h|
+    / 20 away."""
+    from speculative_decode import SpeculativeDecoder
+    decoders = [SpeculativeDecoder(hip_ctx, sequences=5, use_graph=g) for g in (True, False)]
+    d = decoders[0]
+    for _ in range(30):
+        gained = d.step()
+        assert gained == decoders[1].step()
+        h = d.ctx.from_device(d.d_h, (d.rows, d.hidden))
+        logits = d.ctx.from_device(d.d_logits, (d.rows, d.vocab))
+        for r in (0, 15, 16, 19):
+            alone = hip_ctx.gguf_quant_matvec_weight(d.head, d.vocab, d.hidden, h[r])
+            assert np.abs(logits[r] - alone).max() <= 2.0 ** -15 * 1.1 * np.linalg.norm(h[r])
+        p = d.ctx.from_device(d.d_probs, (d.sequences, d.tokens, d.vocab))
+        u = d.ctx.from_device(d.d_uniform, (d.sequences, d.drafts + 1))
+        drafts = d.ctx.from_device(d.d_drafts, (d.sequences, d.drafts), np.uint32)
+        accepted, tokens = R.verify(p, None, drafts, None, u, d.vocab)
+        assert gained == [[int(x) for x in t[:a + 1]] for t, a in zip(tokens, accepted)]
+    for x in decoders:
+        x.close()
