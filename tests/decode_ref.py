@@ -135,14 +135,15 @@ def rotate(x, positions, inv, magnitude, layout):
 
 # ---- attention -----------------------------------------------------------------------
 
-def attention(cache, q, scale, window, counts):
+def attention(cache, q, scale, window, counts, walk=4096):
     """out, its tolerance, weights [sequences][kv_heads][capacity] and theirs.
 
     The tolerance: an f32 score of d terms is off by about 16 units in the last
     place of sum |q k| (d <= 256 roundings, a random walk), which moves p by as
     much on both sides of its fraction; the sums over the slots add a walk of
-    their own, 64 units for up to 4096 slots.
+    their own, 64 units for up to 4096 slots and with the root of `walk` slots above.
     """
+    sums = 64 * max(1.0, walk / 4096) ** 0.5
     b, t, h, d = q.shape
     g = h // cache.kv_heads
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
@@ -166,7 +167,7 @@ def attention(cache, q, scale, window, counts):
                     p /= p.sum()
                     out[s, i, j] = p @ v
                     big = float((np.abs(k) @ np.abs(x)).max()) * abs(scale)
-                    rel = (2 * 16 * big + 64) * 2.0 ** -24
+                    rel = (2 * 16 * big + sums) * 2.0 ** -24
                     tol[s, i, j] = rel * (p @ np.abs(v)) + 1e-30
                     w[s, kv, slots] += p
                     wtol[s, kv, slots] += p * rel + 1e-30

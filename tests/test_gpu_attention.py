@@ -419,3 +419,81 @@ def test_pages_behind_the_window(hip_ctx, dev, kind, page, heads, dim, tokens):
             hip_ctx.synchronize()
         assert "pool" in e.value.message
         check(dev.get(d_out, q), want, tol, policy)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_long_sequences_within_their_sums_walk(hip_ctx, dev, kind):
+    rng = np.random.default_rng(13)
+    c = R.Cache(dev, rng, kind, 4, 1, 64, 64, 626, [40000, 3, 9001, 0])
+    q = (rng.standard_normal((4, 2, 2, 64)) * 2).astype(np.float32)
+    want, tol, _, _ = R.attention(c, q, 0.125, 0, None, walk=40002)
+    for policy in both_policies(hip_ctx):
+        check(attend(hip_ctx, dev, c, q, 0.125), want, tol, policy)
+
+
+@pytest.mark.parametrize("kind,dim,heads,tokens,slots", [
+    ("bf16", 256, 2, 1, 20000), ("f16", 256, 6, 7, 20000), ("f32", 256, 3, 4, 12000),
+    ("f32", 128, 2, 2, 20000), ("bf16", 128, 4, 1, 40000), ("f16", 128, 8, 4, 40000)])
+def test_a_sequence_in_more_shares_than_the_join_loads_at_once(hip_ctx, dev, kind, dim, heads, tokens,
+                                                               slots):
+    """One kv head of one sequence is dealt to some hundred workgroups; a thread of the join holds
+    eight shares of a head of 256 in each of eight groups, or of 128 in sixteen, and takes the
+    others one by one.  Its result, weights too, does not depend on timing."""
+    rng = np.random.default_rng(slots + dim)
+    c = R.Cache(dev, rng, kind, 1, 1, dim, 16, (slots + tokens + 15) // 16, [slots])
+    q = (rng.standard_normal((1, tokens, heads, dim)) * 2).astype(np.float32)
+    scale = float(np.float32(dim ** -0.5))
+    want, tol, w, wtol = R.attention(c, q, scale, 0, None, walk=slots)
+    zero = np.zeros((1, 1, c.capacity), np.float32)
+    first, weights = attend(hip_ctx, dev, c, q, scale, weights=zero)
+    check(first, want, tol)
+    check(weights, w, wtol)
+    for _ in range(3):
+        again, once_more = attend(hip_ctx, dev, c, q, scale, weights=zero)
+        assert np.array_equal(again, first) and np.array_equal(once_more, weights)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kv,group,dim,tokens,lengths", [
+    (32, 1, 64, 1, [2047]),             # eight shares of one sequence
+    (32, 2, 128, 2, [1500, 40, 700]),   # shares that end in sequences and between them
+    (40, 1, 256, 1, [600, 0, 333]),
+    (100, 1, 128, 1, [900, 500]),       # two shares
+    (32, 3, 64, 9, [1100, 200]),        # two row tiles at once
+    (32, 3, 256, 15, [700, 90]),        # three
+    (16, 5, 128, 16, [800, 100]),       # several groups of them
+    (33, 2, 80, 1, [1000, 513]), (12, 6, 80, 7, [900])])
+def test_shares_joined_by_the_last_of_them(hip_ctx, dev, kind, kv, group, dim, tokens, lengths):
+    """Many kv heads leave few shares a sequence; the last one that is done joins them.  Call after
+    call, with and without weights, the counters are back where they were."""
+    rng = np.random.default_rng(kv + dim)
+    heads = kv * group
+    c = R.Cache(dev, rng, kind, len(lengths), kv, dim, 16, (max(lengths) + tokens + 15) // 16, lengths)
+    q = rng.standard_normal((len(lengths), tokens, heads, dim)).astype(np.float32)
+    scale = float(np.float32(dim ** -0.5))
+    want, tol, w, wtol = R.attention(c, q, scale, 0, None)
+    zero = np.zeros((len(lengths), kv, c.capacity), np.float32)
+    first, weights = attend(hip_ctx, dev, c, q, scale, weights=zero)
+    check(first, want, tol)
+    check(weights, w, wtol)
+    assert np.array_equal(attend(hip_ctx, dev, c, q, scale), first)
+    # fewer tokens and a window: other sequences are split, or none
+    counts = np.arange(len(lengths), dtype=np.uint32) % (tokens + 1)
+    want, tol, _, _ = R.attention(c, q, scale, 300, counts)
+    check(attend(hip_ctx, dev, c, q, scale, window=300, counts=counts), want, tol)
+    for _ in range(3):
+        again, once_more = attend(hip_ctx, dev, c, q, scale, weights=zero)
+        assert np.array_equal(again, first) and np.array_equal(once_more, weights)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(10, 2, 80, 16), (6, 1, 96, 32), (8, 2, 192, 16),
+                                               (10, 2, 64, 24), (5, 1, 128, 7), (6, 2, 256, 40)])
+def test_several_row_tiles_at_any_address(hip_ctx, dev, kind, heads, kv, dim, page):
+    rng = np.random.default_rng(heads + dim + page)
+    lengths = [0, 17, 130, 401, 64]
+    c = R.Cache(dev, rng, kind, 5, kv, dim, page, -(-420 // page), lengths)
+    q = rng.standard_normal((5, 11, heads, dim)).astype(np.float32)
+    run(hip_ctx, dev, c, q, weights=True)
+    counts = np.array([11, 4, 0, 9, 1], np.uint32)
+    run(hip_ctx, dev, c, q, window=100, counts=counts, weights=True, what="counts")

@@ -252,3 +252,17 @@ def test_draw_in_steps_of_a_uniform_number(hip_ctx, dev):
                                  vocab)
     assert error is None and not accepted.any()
     assert out[:, 0].tolist() == [17, 17, 17, 4100, 4100, 5000]
+
+
+def test_verify_a_vocabulary_of_many_chunks(hip_ctx, dev):
+    """More chunks of 4096 than a workgroup has threads: each looks for the draw in two."""
+    rng = np.random.default_rng(10)
+    n, m, vocab = 4, 1, (256 + 20) * 4096 + 11
+    target = probabilities(rng, (n, m + 1, vocab), 1.0)
+    draft = probabilities(rng, (n, m, vocab), 1.0)
+    target[2, :, :vocab - 5] = 0.0
+    tokens = rng.integers(0, vocab, (n, m)).astype(np.uint32)
+    uniform = np.array([[0.999, 0.3], [0.999, 0.97], [1.0, 0.6], [0.0, 1 - 2.0 ** -24]], np.float32)
+    for q in (draft, None):
+        _, out, error = check(hip_ctx, dev, target, q, tokens, None, uniform, vocab)
+        assert error is None and out[2, 0] >= vocab - 5

@@ -142,3 +142,17 @@ def test_refuses_to_write_what_it_reads(hip_ctx, dev):
     with pytest.raises(HipError) as e:
         hip_ctx.kv_evict_device(c.handle, w, 32, 8, 0, 0, c.handle, w, 32, w)
     assert e.value.status == -7
+
+
+@pytest.mark.parametrize("n,keep", [(16384, 9000), (16385, 9000), (30001, 20000), (32767, 1),
+                                    (32768, 32767), (32769, 9)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_rows_held_by_a_workgroup(hip_ctx, dev, n, keep, ties):
+    """Around the capacities up to which a thread holds 16 or 32 slots."""
+    rng = np.random.default_rng(n + ties)
+    c = R.Cache(dev, rng, "bf16", 2, 2, 8, 32, -(-n // 32), [n, n // 2 + 1])
+    w = np.exp(rng.standard_normal((2, 2, c.capacity)) * 3).astype(np.float32)
+    if ties:
+        w = np.round(np.log2(w)).astype(np.float32)
+    w[rng.random(w.shape) < 0.1] = 0.0
+    evict(hip_ctx, dev, c, w, keep, min(5, keep - 1), min(64, keep // 2), page=16)
