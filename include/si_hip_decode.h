@@ -137,8 +137,8 @@ int si_hip_kv_advance_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
  * with nothing to attend to (t >= d_counts[s], slots on pages beyond the pool)
  * is zeros.  Slots that a row does not see have no part in it, whatever they
  * hold: NaN and infinities in them do not reach it, and a page before the window
- * may lie beyond the pool.  A row that sees a key or
- * value that is no finite number is not a number, in part or as a whole.
+ * may lie beyond the pool.  A row that sees a key or value that is no finite
+ * number is not a number, in part or as a whole.
  * Sums, maxima and exponentials are f32.  Over an F16 cache a row's query values
  * are held to 22 bits down to 2^-28 of the largest and smaller ones to 2^-51 of it,
  * its p_i to 22 bits down to 2^-17 of the largest and smaller ones to 2^-39 of it;
@@ -150,7 +150,9 @@ int si_hip_kv_advance_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
  * fills anew (refused drafts') are the caller's to clear.
  *
  * d_workspace: si_hip_paged_attention_workspace() bytes of 16-byte aligned
- * device memory that this call may write until it has run. */
+ * device memory that this call may write until it has run.  With d_weights they
+ * hold a score for each row and slot of the capacity, whatever the lengths are:
+ * 4 * sequences * tokens * heads * capacity bytes beside the rest. */
 size_t si_hip_paged_attention_workspace(const si_hip_kv_cache *cache, size_t heads, size_t tokens,
                                         int with_weights); /* 0: invalid arguments */
 int si_hip_paged_attention_device(si_hip_context *ctx, const si_hip_kv_cache *cache, size_t heads,

@@ -118,9 +118,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane, uint32_
 
 // Rounds a share.  Going over to a next sequence takes a workgroup about as long
 // as a round, so a sequence counts for one more, but for the first, where that
-// makes the shares no more than an eighth longer.  (Verified drafts of four
-// sequences 74.5 us without it, 70.2 with it, 74.1 with two rounds; 24 sequences
-// of an f32 cache 110.7, 107.4, 108.2.  But four of 4000 slots, whose 32 shares
+// makes the shares no more than an eighth longer.  (When it was taken, verified
+// drafts of four sequences 74.5 us without it, 70.2 with it, 74.1 with two rounds; 24
+// sequences of an f32 cache 110.7, 107.4, 108.2.  But four of 4000 slots, whose 32 shares
 // of two rounds end where the sequences do, 16.4 without and 20.0 with it.)
 struct Deal {
   uint32_t each, start;

@@ -42,11 +42,11 @@
 //
 // Measured, calls back to back over caches that are not in the L2: one token
 // over 131,071 slots of 4 heads of 256 in BF16 95 us for 537 MB, 5.7 TB/s
-// (6.0 in this kernel), bound by memory; one token a sequence of 24 in F32,
-// 427 MB, 102 us with the weights, of which this kernel has 88; eight drafted
+// (6.1 in this kernel), bound by memory; one token a sequence of 24 in F32,
+// 427 MB, 102 us with the weights, of which this kernel has 89; eight drafted
 // tokens a sequence of four, 183 MB, 58 us, bound by the arithmetic of a round
 // and by what comes before its loads and behind the last (4 us each); one
-// token over 1021 slots of 8 heads of 128, 4.2 MB, 12.4 us: the launch and a
+// token over 1021 slots of 8 heads of 128, 4.2 MB, 12.5 us: the launch and a
 // chain of dependent reads (lengths, page numbers, rows, other shares' sums).
 #pragma once
 
@@ -916,8 +916,9 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
   o.by_tiles = divisor_of(o.tile_groups);
   // A few shares are joined by the last of them; many, whose join is more than
   // one workgroup's work, by a kernel of their own.  (1021 slots of 8 heads of
-  // 128, four shares: 12.9 us inside, 14.8 with the second kernel.  131,071
-  // slots of 4 heads of 256, 64 shares: the second kernel takes 5.5 of 95 us.)
+  // 128, four shares: 1.9 us less inside than with the second kernel, 12.5 in
+  // all.  131,071 slots of 4 heads of 256, 64 shares: the second kernel takes
+  // 5.5 of 95 us.)
   const size_t counters = (size_t)a.cache.sequences * a.cache.kv_heads * o.tile_groups;
   if (o.shares > kSharesJoinedInside || counters * 4u + 64u > kWorkspaceCounterBytes)
     o.counters = nullptr;
@@ -933,9 +934,10 @@ hipError_t launch_mfma(const AttentionArgs& a, Outputs o, hipStream_t s) {
 // once: two, or three where two would leave the last group one of its two; of
 // heads of 128 in 16 bits two, for three of them do not fit the registers (80
 // us instead of 59 for 44 rows over 44,236 slots of 8 heads).  Heads of 256
-// are shared by slots: 48 rows over 44,236 slots of 4 heads 54 us, three tiles
-// at once, where two waves with half of the head each and two tiles at once
-// took 64.
+// are shared by slots: 48 rows over 44,236 slots of 4 heads, three tiles at
+// once, took 54 us where two waves with half of the head each and two tiles at
+// once took 64.  (All four with plain loads of the values, the calls back to
+// back.  Three tiles of F32 heads of 256 spill 30 registers, two none.)
 //
 // Where that is all of the rows, the values' loads are nontemporal (their lines
 // are whole ones; the keys' come in two halves, and measured slower so).  Over
@@ -959,11 +961,11 @@ hipError_t launch_rows(const AttentionArgs& a, const Outputs& o, hipStream_t s) 
   return launch_tiles<T, kDw, kVs, true, 2>(a, o, s);
 }
 
-// Heads of 64, 128 and 256 on pages of whole sixteens take scalar addresses
-// (131,071 slots of 4 heads of 256 100.5 us, 101.3 on pages of 24; heads of 128
-// and F32 alike), and only they leave the registers for several row tiles.  Others take
-// one row tile at a time, in the next larger shape (8 sequences of 4000 slots of
-// 8 heads: 80 values 24.6 us, 96 26.5, 128 30.8).
+// Heads of 64, 128 and 256 on pages of whole sixteens take scalar addresses: only
+// they leave the registers for several row tiles.  (For one it is the same:
+// 131,071 slots of 4 heads of 256 94.5 us, 92.7 on pages of 24; 8 sequences of 4000
+// slots of 8 heads of 128 in F16 31.0 and 30.5.)  Others take one row tile at a time,
+// in the next larger shape (those 8 sequences: 80 values 24.3 us, 96 26.3, 128 31.0).
 template <typename T>
 hipError_t launch_type(const AttentionArgs& a, const Outputs& o, hipStream_t s) {
   const uint32_t dim = a.cache.head_dim;

@@ -112,9 +112,9 @@ __global__ __launch_bounds__(kThreads) void attention_generic(AttentionArgs a, f
 }
 
 // weights[slot] += sum over the kv head's rows of exp2(score - m) / l.  grid
-// (blocks of 256 / PARTS slots, from `first_block` on, kv_heads, sequences): the waves
-// of a workgroup add up 1 / PARTS of the rows each, in their order, kAhead rows' loads under way at
-// once; the parts are added in theirs.  Up to eight rows are one part, more
+// (blocks of 256 / PARTS slots, from `first_block` on, kv_heads, sequences): the
+// waves of a workgroup add up 1 / PARTS of the rows each, in their order, kAhead
+// rows' loads under way at once; the parts are added in theirs.  Up to eight rows are one part, more
 // four (24 sequences of 2000 slots, four rows a head: with the attention 96.4
 // us in one part, 106.3 in four; 25 of 65 slots, 112 rows: 47.9 and 39.1, 72.1
 // row by row).

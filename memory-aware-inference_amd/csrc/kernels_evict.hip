@@ -10,8 +10,8 @@
 // threads read their slots, next to each other, once and hold them (up to 32768
 // slots; more are read in each pass), and one scan over the threads places all
 // that is kept.  Measured: 4 heads of 4111 slots of 256 values, 3001 kept,
-// 16.3 us (selection 9.5, move 6) for 24.8 MB; 64 heads of up to 16,384 slots of
-// 128, 6144 kept, 94 us (16 and 77) for 379 MB, the move at 4.9 TB/s read and
+// 15.9 us (selection 10, move 6) for 24.8 MB; 64 heads of up to 16,384 slots of
+// 128, 6144 kept, 94 us (17 and 77) for 379 MB, the move at 4.9 TB/s read and
 // written.
 #include "decode_internal.h"
 
@@ -311,8 +311,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs a, uint32_t
 hipError_t launch_evict(const EvictArgs& a, hipStream_t s) {
   const CacheView& c = a.from;
   const dim3 heads(c.kv_heads, c.sequences);
-  // (4 heads of 4111 slots, selection and move: held in a place of 16,384 14.4 us, of 32,768
-  // 16.5, read in each pass 16.7; 64 heads of 30,000 slots: held 102 us, read 117.)
+  // (Selection and move of 4 heads of 4111 slots of 256: held in a place of 16,384 15.9 us, of
+  // 32,768 17.0, read in each pass 17.5; 64 heads of 30,000 slots of 16: held 70 us, read 96.)
   if (c.capacity <= 16u * kThreads)
     evict_select<16><<<heads, kThreads, 0, s>>>(a);
   else if (c.capacity <= 32u * kThreads)

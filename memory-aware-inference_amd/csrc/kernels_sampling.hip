@@ -48,7 +48,7 @@ __device__ __forceinline__ void load_fours(const float* row, size_t base, size_t
 // maximum and sum (scratch), once, with the row's from all of them, for y.  288
 // rows of 151,936 logits: 81 us, 31 and 50, for 350 MB read, read again (half
 // of it from the caches) and written, 4.3 TB/s of what has to move once; 5 rows
-// 7.5 us, two launches of little more than an empty one.
+// 7.6 us, two launches of little more than an empty one.
 
 // (maximum, sum of exp2((x - maximum) per)) of two parts of a row; `per` is
 // log2(e) / T.  The difference is taken first, so its rounding is that of a
@@ -394,7 +394,7 @@ hipError_t launch_softmax(const float* x, float* y, size_t rows, size_t cols, fl
   const float per = kLog2e / temperature;
   // Chunks of 8192 values where they make a workgroup a CU, else of 2048, so that a few rows
   // have more of them (of 151,936 logits 24 rows 10.1 us by 8192 and 12.0 by 2048, 16 rows
-  // 9.8 both; 5 rows 7.0 by 2048).
+  // 9.8 both; 5 rows 7.6 by 2048).
   const bool many = rows * ((cols + 8191u) / 8192u) >= 256u;
   return many ? softmax_rows<8>(x, y, rows, cols, per, ws, s)
               : softmax_rows<2>(x, y, rows, cols, per, ws, s);
