@@ -321,8 +321,6 @@ def prepare(case, seed):
                 sequences=case["sequences"], max_pages=c["table"].shape[1],
                 d_keys=c["keys"].data_ptr(), d_values=c["values"].data_ptr(),
                 d_page_table=c["table"].data_ptr(), d_lengths=c["lengths"].data_ptr())
-        if kind == "conv":
-            s["activation"] = si_hip.CONV_SILU if case["silu"] else si_hip.CONV_NONE
         if kind == "scan":
             s["scan"] = si_hip.StateScan(
                 rule=RULES.index(case["rule"]), head_order=ORDERS.index(case["order"]),
@@ -485,10 +483,11 @@ def run(state):
             q_token_stride=q.stride(1), q_head_stride=q.stride(2), d_q_out=at(s["out"]))
         return {"q": s["out"], "keys": s["cache"]["keys"], "values": s["cache"]["values"]}
     if kind == "conv":
+        si_hip = _package()
         ctx.causal_conv_device(
             at(s["x"]), at(s["weight"]), case["sequences"], case["tokens"], case["channels"],
             case["width"], d_y=at(s["out"]), d_bias=at(s["bias"]),
-            activation=s["activation"],
+            activation=si_hip.CONV_SILU if case["silu"] else si_hip.CONV_NONE,
             d_state=at(s["state"]), d_state_out=at(s["new_state"]), d_counts=at(s["counts"]))
         return {"out": s["out"], "state": s["new_state"]}
     x, n = s["qkv"], case["key_heads"] * case["key_dim"]
