@@ -20,8 +20,9 @@
 // to their length or largest value, of a state's column and of what it gains, both to their largest
 // value, there 21 without the correction; three products of pieces).  R, U and what they are multiplied by are three bf16 each (8
 // bits of each, cut off, so that their sum is the value; six products): a loud token that is
-// forgotten within its chunk costs the quiet ones behind it nothing.  The sums G are 64 bits wide: the
-// difference of two of them is as exact as the gates.
+// forgotten within its chunk costs the quiet ones behind it nothing.  The sums G are 64 bits wide, of
+// log decays of no less than -256: they stay below 2^14 and good to 2^-38, so that the difference of two of them is as
+// exact as the gates.
 //
 // A chunk of one workgroup by itself is a chain: products with the state, the system's three products,
 // P's, the units, the state's own; a taker's wave, alone on its SIMD, issues or waits for one of
@@ -49,6 +50,7 @@ constexpr uint32_t kChunk = 32;
 constexpr uint32_t kPieces = 3;       // bf16
 constexpr uint32_t kHalves = 2;       // f16
 constexpr float kUp = 0x1p14f;        // what keys and queries are held times
+constexpr float kForgotten = -256.0f; // the least log decay of a token
 // The waves of a workgroup: `takers` that take sixteen columns each through the chunks, two or four that
 // make the rows of K and Q, and two that make what is left of a chunk's operands.  Four makers of
 // rows where two takers leave registers for eight waves: theirs is the longest course without the
@@ -367,7 +369,9 @@ __device__ __forceinline__ void make_gates(ChunkShared<STEPS>& sh, uint32_t n, c
   if (lane < left && lane < kChunk) {
     const float s = softplus(gate + bias);
     log_keep = decay * s;
-    if (log_keep < -3.0e38f) log_keep = -3.0e38f;  // (the differences of sums stay numbers)
+    // (e^-256 is zero in f32, and so is every factor across this token; what is larger would cost the
+    // sums behind it the bits of their own tokens' decays, an infinite one all of them)
+    if (log_keep < kForgotten) log_keep = kForgotten;
     write = DELTA ? sigmoid(beta) : s;
   }
   double sum = log_keep * 1.4426950408889634;

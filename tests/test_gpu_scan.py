@@ -1,4 +1,6 @@
 """GPU: the state scan against 64 bits (tolerances: mixer_ref.Scan)."""
+import copy
+
 import numpy as np
 import pytest
 
@@ -428,3 +430,34 @@ def test_rows_behind_2_to_32(hip_ctx, dev):
     hip_ctx.synchronize()
     check_out(dev.get(d_out, o), out, out_tol)
     within(dev.get(scan.d_state, st), state, state_tol, "state")
+
+
+@pytest.mark.parametrize("gate", [1e9, 1e12, 1e14, 1e16, 1e30, 3e38, np.inf])
+@pytest.mark.parametrize("rule", [DELTA, SELECTIVE])
+@pytest.mark.parametrize("tokens,at,dk", [(3, 1, 64), (12, 3, 64), (70, 40, 128), (70, 37, 160)])
+def test_gates_that_clear_the_state(hip_ctx, dev, tokens, at, dk, rule, gate):
+    """A gate so large that nothing before its token is left, in the middle of a chunk, and ordinary ones
+    behind it: what follows is a sequence that begins there, without a state.  (So the reference's first
+    token needs no such gate; the selective form's step multiplies the value, too, which is made that
+    much smaller, and so rounded once more, and has no product with an infinite one.)"""
+    if rule == SELECTIVE and gate == np.inf:
+        pytest.skip("its step times a value is no finite number")
+    scan = M.Scan(np.random.default_rng(41), 2, tokens, 1, 3, dk, 48, rule)
+    whole = scan.run()
+    rest = copy.copy(scan)
+    rest.shape = (2, tokens - at) + scan.shape[2:]
+    for name in ("q", "k", "v", "gate", "beta"):
+        x = getattr(scan, name)
+        setattr(rest, name, None if x is None else x[:, at:].copy())
+    rest.state = None
+    rest.gate[:, 0] = 0.0
+    scan.gate[:, at] = gate
+    if rule == SELECTIVE:
+        scan.v[:, at] /= np.float32(gate)
+        step = np.logaddexp(0.0, rest.bias.astype(np.float64))
+        rest.v[:, 0] = (scan.v[:, at].astype(np.float64) * np.float64(np.float32(gate)) / step[:, None])
+    out, out_tol, state, state_tol = rest.run(chunked=tokens >= 4)
+    got, new = run(hip_ctx, dev, scan)
+    within(got[:, :at], whole[0][:, :at], whole[1][:, :at], "out before")
+    within(got[:, at:], out, out_tol, "out behind")
+    within(new, state, state_tol, "state")
