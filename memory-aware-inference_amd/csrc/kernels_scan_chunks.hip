@@ -31,7 +31,9 @@
 // vector instructions of four cycles and more and 230 matrix instructions of 16: 9 thousand cycles.
 //
 // What is no finite number stays where it belongs: a zero of L or P times a later token's NaN
-// would not, so a wave that finds one in U takes the chunk token by token.
+// would not, so a wave that finds one in U takes the chunk token by token.  So do all of them where a key or query is
+// so short beside eps's root that its pieces, held over its length, would lose bits: its row is raised
+// by a power of two that is kept beside it.
 #include "scan_common.h"
 
 namespace sihip {
@@ -183,6 +185,7 @@ struct Gated {  // of a chunk's tokens
   float keep[kChunk];   // a_i
   float key[kChunk], query[kChunk];  // what the rows of the operands are to be multiplied by
   float total;          // e^{G}
+  alignas(4) uint8_t raised[4];  // of eight rows each: whether some are raised, and all have key[], query[] (delta rule)
 };
 
 // Keys of more than 128 values leave room for fewer chunks: rows of two, blocks of one.  Then a chunk's
@@ -305,8 +308,10 @@ __device__ __forceinline__ void each(F f) {
   }
 }
 
-// Keys and queries in pieces: under the delta rule of length 1, else to a power of two that
-// is kept beside them.
+// Keys and queries in pieces: under the delta rule over their length, else to a power of two that
+// is kept beside them.  Over its length a row of the length l is l / sqrt(l^2 + eps) long: where that is 2^-12 and
+// more, its largest value is held as 2^-2 at least, and f16's least step, 2^-24, is 22 bits of it.  Shorter
+// rows are raised.
 template <uint32_t STEPS, bool DELTA, uint32_t MAKERS>
 __device__ __forceinline__ void make_rows(ChunkShared<STEPS>& sh, uint32_t chunk,
                                           const Raw<STEPS, MAKERS>& r, const ScanArgs& a, uint32_t part,
@@ -317,29 +322,45 @@ __device__ __forceinline__ void make_rows(ChunkShared<STEPS>& sh, uint32_t chunk
   const uint32_t at = 4u * in, step = at / 32u, half = at / 16u % 2u, p = at / 4u % 4u;
   const bool held = at < 32u * STEPS;
   float x[V], scale;
+  Gated& g = sh.gated[chunk % 3u];
+  auto sizes = [&] {
 #pragma unroll
-  for (uint32_t l = 0; l < W::kLoads; ++l) {
-    if (DELTA) {
+    for (uint32_t l = 0; l < W::kLoads; ++l) {
+      x[2 * l] = largest(r.k[l], 0.0f);
+      x[2 * l + 1] = largest(r.q[l], 0.0f);
+    }
+    return reduced<W::kLanes>(x, lane, [](float y, float z) { return fmaxf(y, z); });
+  };
+  const uint32_t token = row + in % V / 2u * W::kRows;  // of the value that comes to this lane
+  if (DELTA) {
+#pragma unroll
+    for (uint32_t l = 0; l < W::kLoads; ++l) {
       auto squares = [](const f32x4& y) {
         return __builtin_fmaf(y[3], y[3], __builtin_fmaf(y[2], y[2], __builtin_fmaf(y[1], y[1], y[0] * y[0])));
       };
       x[2 * l] = squares(r.k[l]);
       x[2 * l + 1] = squares(r.q[l]);
-    } else {
-      x[2 * l] = largest(r.k[l], 0.0f);
-      x[2 * l + 1] = largest(r.q[l], 0.0f);
     }
-  }
-  const uint32_t token = row + in % V / 2u * W::kRows;  // of the value that comes to this lane
-  if (DELTA) {
     const float sum = reduced<W::kLanes>(x, lane, [](float y, float z) { return y + z; });
     // (rows behind the last token are zeros whatever eps is)
     scale = kUp * inverse_root(sum + (token < left ? a.eps : 1.0f));
+    bool small = token < left && sum < a.eps * 0x1p-24f;
+    bool some = false;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(small) != 0u, 0)) {
+      const float most = sizes();
+      small = small && most > 0.0f;  // (zeros are held as they are)
+      some = __builtin_amdgcn_ballot_w64(small) != 0u;
+      // (the largest into [2^12, 2^14); what is below 2^-112, or 2^-114 of its length, has fewer bits)
+      const int32_t e = exponent(scale);
+      const int32_t up = small ? max(min(min(266 - exponent(most) - e, 253 - e), 126), 0) : 0;
+      scale *= __uint_as_float((uint32_t)(127 + up) << 23);
+      if (in < V) (in % 2u ? g.query : g.key)[token] = __uint_as_float((uint32_t)(127 - up) << 23);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < W::kPartRows / 8u; ++i) g.raised[part * (W::kPartRows / 8u) + i] = some;
   } else {
     float down;
-    scale = scale_of(reduced<W::kLanes>(x, lane, [](float y, float z) { return fmaxf(y, z); }),
-                     &down);
-    Gated& g = sh.gated[chunk % 3u];
+    scale = scale_of(sizes(), &down);
     if (in < V) (in % 2u ? g.query : g.key)[token] = in % 2u ? a.scale * down : down;
   }
   auto put = [&](u32x4* to, const f32x4& y, uint32_t t) {
@@ -615,7 +636,9 @@ __device__ void take_steps(State<STEPS>& st, const ChunkShared<STEPS>& sh, uint3
     const float v = __uint_as_float(
         __builtin_amdgcn_raw_buffer_load_b32(from, v_at + t * 4u * (uint32_t)c.v_stride, 0, 0));
     const float keep = g.keep[t], write = g.write[t];
-    const float kf = DELTA ? 1.0f / kUp : g.key[t], qf = DELTA ? qscale / kUp : g.query[t];
+    const bool factors = !DELTA || g.raised[t / 8u];
+    const float kf = (factors ? g.key[t] : 1.0f) * (DELTA ? 1.0f / kUp : 1.0f);
+    const float qf = (factors ? g.query[t] : 1.0f) * (DELTA ? qscale / kUp : 1.0f);
     float sk = 0.0f, sq = 0.0f;
 #pragma unroll
     for (uint32_t k = 0; k < 2 * STEPS; ++k) {
@@ -769,12 +792,14 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
     put(u[0], 0u);
     put(u[1], 1u);
   }
-  bool odd = false;
+  bool odd = DELTA && *reinterpret_cast<const uint32_t*>(g.raised);
 #pragma unroll
   for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) odd |= __builtin_amdgcn_classf(u[t][i], 0x207);  // NaN, infinity
-  if (__builtin_amdgcn_ballot_w64(odd)) {
+  // (the steps' code goes behind the rest where that leaves registers: 9.85 against 11.0 us for a call of one chunk)
+  const bool steps = __builtin_amdgcn_ballot_w64(odd) != 0u;
+  if (DELTA && STEPS <= 4 ? __builtin_expect(steps, false) : steps) {
     take_steps<STEPS, DELTA>(st, sh, chunk, c, t0, left, lane, qscale, skip);
     return;
   }

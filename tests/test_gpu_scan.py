@@ -461,3 +461,30 @@ def test_gates_that_clear_the_state(hip_ctx, dev, tokens, at, dk, rule, gate):
     within(got[:, :at], whole[0][:, :at], whole[1][:, :at], "out before")
     within(got[:, at:], out, out_tol, "out behind")
     within(new, state, state_tol, "state")
+
+
+@pytest.mark.parametrize("eps", [1e-6, 1.0])
+@pytest.mark.parametrize("size", [1e-4, 1e-7, 1e-9, 1e-12, 1e-20, 1e-30])
+@pytest.mark.parametrize("tokens,dk,which", [(6, 64, "q"), (40, 128, "q"), (40, 160, "q"), (6, 64, "k"),
+                                             (40, 128, "k"), (70, 33, "k"), (40, 160, "k"), (70, 64, "qk")])
+def test_short_rows(hip_ctx, dev, tokens, dk, which, size, eps):
+    """Keys and queries far shorter than eps's root, some of them or all of a chunk's, zeros among them: their
+    products are as exact as longer ones', to the least numbers of f32 and their products."""
+    rng = np.random.default_rng(43)
+    scan = M.Scan(rng, 2, tokens, 2, 4, dk, 40)
+    scan.eps = eps
+    scan.gate -= 2.0
+    rows = np.ones(tokens, bool)
+    if tokens != 40:
+        rows[1::3] = False
+    for name in which:
+        x = getattr(scan, name)
+        x[:, rows] *= np.float32(size)
+        x[:, 3] = 0.0
+    if "k" in which:  # so that what such keys leave is what the outputs are made of
+        scan.state[:] = 0.0
+        scan.v *= np.float32(min(1.0 / size, 1e12))
+    out, out_tol, state, state_tol = scan.run()
+    got, new = run(hip_ctx, dev, scan)
+    check_out(got, out, out_tol)
+    within(new, state, state_tol, "state")
