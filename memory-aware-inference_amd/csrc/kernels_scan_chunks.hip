@@ -178,14 +178,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const float* first, si
   return buffer_of(first, min(left, kChunk) * (uint32_t)stride * 4u);
 }
 
-struct Gated {  // of a chunk's tokens
+struct alignas(16) Gated {  // of a chunk's tokens (four of them are read at once)
   float grow[kChunk];   // e^{G_i}
   float fade[kChunk];   // e^{G - G_i}
   float write[kChunk];  // w_i
   float keep[kChunk];   // a_i
   float key[kChunk], query[kChunk];  // what the rows of the operands are to be multiplied by
   float total;          // e^{G}
-  alignas(4) uint8_t raised[4];  // of eight rows each: whether some are raised, and all have key[], query[] (delta rule)
+  // of eight rows each: whether some are raised, and all have key[], query[] (delta rule)
+  alignas(4) uint8_t raised[4];
 };
 
 // Keys of more than 128 values leave room for fewer chunks: rows of two, blocks of one.  Then a chunk's
