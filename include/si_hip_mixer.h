@@ -85,7 +85,7 @@ typedef struct si_hip_state_scan {
  *
  * States, sums and decays are f32, or wider.  Single tokens, and rows more than 2^23
  * floats apart, are taken token by token in f32; prompts and most calls of four
- * tokens and more in chunks of 32 on the matrix cores, each f32 operand as a sum of two f16 (21 bits or more of the
+ * tokens and more in chunks of 32 on the matrix cores, each f32 operand as a sum of two f16 (22 bits of the
  * largest value of its row or column) or three bf16 (all of its bits).  What a chunk forgets
  * to less than 2^-126 of it within 32 tokens counts as forgotten, and none grows to 2^127 times what it was. */
 int si_hip_state_scan_device(si_hip_context *ctx, const si_hip_state_scan *scan, size_t sequences,

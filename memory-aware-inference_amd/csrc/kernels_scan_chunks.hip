@@ -17,8 +17,8 @@
 //
 // The matrix cores take 16-bit operands, f32 values as sums of pieces.  Products of whole columns,
 // whose errors count against a column's size, are of two f16 each (22 bits of keys and queries,
-// to their length or largest value, of a state's column and of what it gains, both to their largest
-// value, there 21 without the correction; three products of pieces).  R, U and what they are multiplied by are three bf16 each (8
+// to their largest value, of a state's column and of what it gains, both to the larger of their largest
+// values; three products of pieces).  R, U and what they are multiplied by are three bf16 each (8
 // bits of each, cut off, so that their sum is the value; six products): a loud token that is
 // forgotten within its chunk costs the quiet ones behind it nothing.  The sums G are 64 bits wide, of
 // log decays of no less than -256: they stay below 2^14 and good to 2^-38, so that the difference of two of them is as
@@ -51,7 +51,10 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kChunk = 32;
 constexpr uint32_t kPieces = 3;       // bf16
 constexpr uint32_t kHalves = 2;       // f16
-constexpr float kUp = 0x1p14f;        // what keys and queries are held times
+// What keys and queries are held times: far enough above f16's least numbers for their low pieces, and what is
+// added to a state as far, which is held in its units over this (2^14 left those 2^-22 to 2^-21 of the
+// largest, and states of the selective form 2.3e-7 to 2.7e-7 off where now 1.4e-7).
+constexpr float kUp = 0x1p10f;
 constexpr float kForgotten = -256.0f; // the least log decay of a token
 // The waves of a workgroup: `takers` that take sixteen columns each through the chunks, two or four that
 // make the rows of K and Q, and two that make what is left of a chunk's operands.  Four makers of
@@ -112,11 +115,11 @@ __device__ __forceinline__ void halve8(const f32x4& lo, const f32x4& hi, u32x4 (
 #pragma unroll
   for (uint32_t i = 0; i < kHalves; ++i) p[i] = u32x4{w[0][i], w[1][i], w[2][i], w[3][i]};
 }
-// The power of two that takes a largest value m (of at least 2^-112) into [2^14, 2^15), and its inverse.
+// The power of two that takes a largest value m (of at least 2^-119) into [2^7, 2^8), and its inverse.
 __device__ __forceinline__ float scale_of(float m, float* inverse) {
-  const uint32_t e = min(max(__float_as_uint(m) >> 23, 15u), 254u);
-  *inverse = __uint_as_float((e - 14u) << 23);
-  return __uint_as_float((268u - e) << 23);
+  const uint32_t e = min(max(__float_as_uint(m) >> 23, 8u), 254u);
+  *inverse = __uint_as_float((e - 7u) << 23);
+  return __uint_as_float((261u - e) << 23);
 }
 __device__ __forceinline__ int32_t exponent(float x) {  // of x >= 0, biased
   return (int32_t)(__float_as_uint(x) >> 23);
@@ -310,7 +313,7 @@ __device__ __forceinline__ void each(F f) {
 }
 
 // Keys and queries in pieces: under the delta rule over their length, else to a power of two that
-// is kept beside them.  Over its length a row of the length l is l / sqrt(l^2 + eps) long: where that is 2^-12 and
+// is kept beside them.  Over its length a row of the length l is l / sqrt(l^2 + eps) long: where that is 2^-8 and
 // more, its largest value is held as 2^-2 at least, and f16's least step, 2^-24, is 22 bits of it.  Shorter
 // rows are raised.
 template <uint32_t STEPS, bool DELTA, uint32_t MAKERS>
@@ -345,15 +348,15 @@ __device__ __forceinline__ void make_rows(ChunkShared<STEPS>& sh, uint32_t chunk
     const float sum = reduced<W::kLanes>(x, lane, [](float y, float z) { return y + z; });
     // (rows behind the last token are zeros whatever eps is)
     scale = kUp * inverse_root(sum + (token < left ? a.eps : 1.0f));
-    bool small = token < left && sum < a.eps * 0x1p-24f;
+    bool small = token < left && sum < a.eps * 0x1p-16f;
     bool some = false;
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(small) != 0u, 0)) {
       const float most = sizes();
       small = small && most > 0.0f;  // (zeros are held as they are)
       some = __builtin_amdgcn_ballot_w64(small) != 0u;
-      // (the largest into [2^12, 2^14); what is below 2^-112, or 2^-114 of its length, has fewer bits)
+      // (the largest into [2^8, 2^10); what is below 2^-118 has fewer bits)
       const int32_t e = exponent(scale);
-      const int32_t up = small ? max(min(min(266 - exponent(most) - e, 253 - e), 126), 0) : 0;
+      const int32_t up = small ? max(min(min(262 - exponent(most) - e, 253 - e), 126), 0) : 0;
       scale *= __uint_as_float((uint32_t)(127 + up) << 23);
       if (in < V) (in % 2u ? g.query : g.key)[token] = __uint_as_float((uint32_t)(127 - up) << 23);
     }
@@ -873,7 +876,7 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
   const float rest = all * most;
   gained = columns_max(gained);
   const int32_t size =
-      max(exponent(rest), exponent(gained) - exponent(st.unit) + (DELTA ? 127 : 142));
+      max(exponent(rest), exponent(gained) - exponent(st.unit) + (DELTA ? 127 : 135));
   const bool some = rest > 0.0f || gained > 0.0f;
   if (__builtin_amdgcn_ballot_w64(some && !st.fits(size))) {
     // (the state is multiplied once, by both: what is forgotten may not fit the new units)
