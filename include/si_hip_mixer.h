@@ -13,7 +13,10 @@
  * only min(d_counts[s] + more, tokens) of them; the rows behind are not read
  * and their outputs stay as they were.  d_state NULL: sequences begin (their
  * state is zero).  d_state_out may be d_state, or NULL: the new state is not
- * kept.  The outputs may be NULL where only the state is wanted.  So drafted
+ * kept.  The outputs may be NULL where only the state is wanted.  An output
+ * that shares memory with an input, a parameter or another output is refused, but for
+ * d_state_out = d_state; what lies between the rows of a strided argument is none
+ * of it.  So drafted
  * tokens are verified without touching the state, and when it is known how many were
  * accepted a second call with d_counts = the accepted and more = 1 (for the
  * token before them) takes the state that far. */
@@ -38,7 +41,7 @@ extern "C" {
  * convolution of each channel by itself; inputs before the first token are the
  * state, [sequences][width - 1][channels], the oldest first.  2 <= width <=
  * SI_HIP_MAX_CONV_WIDTH; d_bias NULL: none.  Rows are x_token_stride / y_token_stride floats
- * apart.  d_y must not overlap d_x.  A token's output depends on its own and the
+ * apart.  A token's output depends on its own and the
  * width - 1 inputs before it alone. */
 int si_hip_causal_conv_device(si_hip_context *ctx, size_t sequences, size_t tokens,
                               const uint32_t *d_counts, uint32_t more, size_t channels,

@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "mixer_internal.h"
+#include "overlap.h"
 #include "si_hip_status.h"
 
 using namespace sihip;
@@ -67,7 +68,15 @@ int si_hip_causal_conv_device(si_hip_context *ctx, size_t sequences, size_t toke
   if (d_y && (rc = check_stride(y_token_stride, channels, "causal convolution")) != 0) return rc;
   if (!ctx || !d_x || !d_weight || (!d_y && !d_state_out))
     return set_error(SI_HIP_ERR_NULL, "device causal convolution argument is null");
-  if (d_x == d_y || d_state_out == d_x || (d_y && (d_y == d_state || d_y == d_state_out)))
+  const size_t rows = sequences * tokens, held = sequences * (width - 1);
+  const Region y(d_y, rows, 4 * y_token_stride, 4 * channels);
+  const Region state(d_state, held, 4 * channels, 4 * channels);
+  const Region state_out(d_state_out, held, 4 * channels, 4 * channels);
+  const Region in[] = {Region(d_x, rows, 4 * x_token_stride, 4 * channels),
+                       Region(d_weight, channels, 4 * width, 4 * width),
+                       Region(d_bias, 4 * channels), Region(d_counts, 4 * sequences)};
+  if (overlaps_any(y, in) || overlaps_any(state_out, in) || overlap(y, state) ||
+      overlap(y, state_out) || (d_state_out != d_state && overlap(state_out, state)))
     return set_error(SI_HIP_ERR_RANGE, "causal convolution writes what it reads");
   const ConvArgs a{(uint32_t)sequences,
                    (uint32_t)channels,

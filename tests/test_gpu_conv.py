@@ -144,3 +144,22 @@ def test_more_runs_than_a_launch_has(hip_ctx, dev, channels):
     # (three roundings of at most half a step: two products and their sum)
     assert np.all(np.abs(dev.get(d_y, x)[0] - want) <= 1.1 * 3 * M.U * size + 1e-36)
     assert np.array_equal(dev.get(d_out, state)[0], x[0, -1:])
+
+
+def test_rows_beside_one_another(hip_ctx, dev):
+    """Inputs and outputs in the same rows of one buffer, each between the other's."""
+    rng = np.random.default_rng(6)
+    n, tokens, channels, width = 2, 70, 40, 4
+    x, w, b, state = inputs(rng, n, tokens, channels, width, True, False)
+    rows = np.full((n, tokens, 2 * channels + 3), 9.0, np.float32)
+    rows[..., channels + 2:2 * channels + 2] = x
+    want, tol, states = M.conv(x, w, b, state, [tokens] * n, 1)
+    d, d_state = dev.put(rows), dev.put(state)
+    hip_ctx.causal_conv_device(d + 4 * (channels + 2), dev.put(w), n, tokens, channels, width, d_y=d + 4,
+                               d_bias=dev.put(b), d_state=d_state, d_state_out=d_state,
+                               x_token_stride=2 * channels + 3, y_token_stride=2 * channels + 3)
+    hip_ctx.synchronize()
+    got = dev.get(d, rows)
+    check(got[..., 1:channels + 1], want, tol)
+    got[..., 1:channels + 1] = 9.0
+    assert np.array_equal(got, rows) and np.array_equal(dev.get(d_state, states), states)

@@ -1,6 +1,8 @@
 """CPU: refusals of a hybrid decoder layer's mixers (include/si_hip_mixer.h, the head norms and
 several-axis positions of include/si_hip_decode.h), each before the context is looked at, and the
 table of axes."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -140,3 +142,47 @@ def test_scan():
                  dict(out=None, state_out=None)):
         assert scan(**more) == NULL
     # (with a context those are refused, too: the outputs are none of the inputs)
+
+
+# Refusals of outputs that share memory with what a call reads come last, so they need a context: this one is
+# never looked at.
+FAKE = C.create_string_buffer(1 << 16)
+CONTEXT = C.addressof(FAKE)
+ROOM = 1 << 20  # bytes between arguments that share nothing
+
+
+def shared(status):
+    return status == RANGE and "writes what it reads" in si_hip.last_error()
+
+
+CONV = dict(sequences=3, tokens=5, counts=2, channels=40, width=4, xs=90, ys=100)
+
+
+def conv_at(**more):
+    a = {**{k: ROOM * (i + 1) for i, k in enumerate(("x", "w", "b", "state", "out", "y", "n"))}, **CONV, **more}
+    return si_hip.lib().si_hip_causal_conv_device(
+        CONTEXT, a["sequences"], a["tokens"], a["n"], 0, a["channels"], a["width"], a["x"], a["xs"], a["w"], a["b"],
+        1, a["state"], a["out"], a["y"], a["ys"])
+
+
+SIZES = dict(x=4 * (14 * 90 + 40), w=4 * 160, b=160, state=4 * 9 * 40, n=12)
+
+
+@pytest.mark.parametrize("read", ["x", "w", "b", "state", "n"])
+@pytest.mark.parametrize("written,size", [("y", 4 * (14 * 100 + 40)), ("out", 4 * 9 * 40)])
+def test_conv_outputs_apart(read, written, size):
+    """At the first byte that is shared and the last, from either side."""
+    at = 64 * ROOM
+    for where in (at, at + 4, at + SIZES[read] - 4, at - size + 4):
+        if (read, written, where) != ("state", "out", at):
+            assert shared(conv_at(**{read: at, written: where})), where
+    assert shared(conv_at(y=at, out=at + 4 * 14 * 100))
+
+
+def test_conv_in_one_buffer():
+    """Rows beside one another in wider ones: a channel that both have, and outputs of another row length."""
+    at = 64 * ROOM
+    for y in (at + 4 * 39, at + 4 * 91, at + 4 * 90 * 3 - 4, at - 4):
+        assert shared(conv_at(x=at, y=y, ys=90))
+    assert shared(conv_at(x=at, y=at + 4 * 50, ys=100)) and shared(conv_at(x=at, y=at + 4 * 45, ys=91))
+    assert shared(conv_at(x=at, out=at + 4 * 40, channels=40))

@@ -1,0 +1,67 @@
+"""CPU: whether two strided arguments share memory (csrc/overlap.h), against a count of their bytes."""
+import subprocess
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parent.parent / "memory-aware-inference_amd" / "csrc"
+
+PROGRAM = r"""
+#include "overlap.h"
+#include <cstdio>
+#include <vector>
+using sihip::Region;
+static uint32_t state = 1;
+static uint32_t below(uint32_t n) {
+  state = state * 1664525u + 1013904223u;
+  return (state >> 8) % n;
+}
+constexpr uintptr_t kBase = 0x1000;
+static Region some(uint32_t same_block, uint32_t same_row) {
+  const uint32_t size = 1 + below(6), rows = 1 + below(4), blocks = 1 + below(5);
+  const uint32_t row_stride = std::max(size, same_row ? same_row : size + below(8));
+  const uint32_t span = (rows - 1) * row_stride + size;
+  const uint32_t block_stride = std::max(span, same_block ? same_block : span + below(20));
+  return Region((void*)(kBase + below(60)), blocks, block_stride, rows, row_stride, size);
+}
+int main() {
+  unsigned long shared = 0, interlocked = 0;
+  for (int n = 0; n < 400000; ++n) {
+    const Region a = some(n % 3 == 1 ? 24 : 0, n % 2 ? 6 : 0), b = some(n % 3 == 1 ? 24 : 0, n % 2 ? 6 : 0);
+    std::vector<char> bytes(4096, 0);
+    bool want = false;
+    for (int pass = 0; pass < 2; ++pass) {
+      const Region& r = pass ? b : a;
+      for (size_t i = 0; i < r.blocks; ++i)
+        for (size_t j = 0; j < r.rows; ++j)
+          for (size_t k = 0; k < r.size; ++k) {
+            char& x = bytes[r.at - kBase + i * r.block_stride + j * r.row_stride + k];
+            if (pass) want |= x;
+            else x = 1;
+          }
+    }
+    shared += want;
+    interlocked += !want && a.at < b.end && b.at < a.end;
+    if (sihip::overlap(a, b) != want || sihip::overlap(b, a) != want) {
+      std::printf("wrong for case %d\n", n);
+      return 1;
+    }
+  }
+  // none, the whole address space, more rows than a loop could take
+  const Region none(nullptr, 8), all((void*)16, size_t(1) << 40, size_t(1) << 40, 4);
+  const Region q((void*)0x10000, size_t(1) << 31, 3072, 1024), k((void*)0x10400, size_t(1) << 31, 3072, 2048);
+  const Region over((void*)0x10400, size_t(1) << 31, 3072, 2049);
+  if (sihip::overlap(none, all) || sihip::overlap(all, none) || !sihip::overlap(all, all) ||
+      sihip::overlap(q, k) || !sihip::overlap(q, over) || all.end != UINTPTR_MAX)
+    return 2;
+  std::printf("%lu shared, %lu interlocked\n", shared, interlocked);
+  return shared > 1000 && interlocked > 1000 ? 0 : 3;
+}
+"""
+
+
+def test_overlap(tmp_path):
+    src, exe = tmp_path / "overlap.cpp", tmp_path / "overlap"
+    src.write_text(PROGRAM)
+    subprocess.run(["/opt/rocm/bin/hipcc", "--cuda-host-only", "-std=c++17", "-O1", f"-I{CSRC}", str(src), "-o",
+                    str(exe)], check=True, timeout=300)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stdout
