@@ -127,11 +127,19 @@ int si_hip_state_scan_device(si_hip_context *ctx, const si_hip_state_scan *scan,
   if (!ctx || !scan->d_decay || !d_k || !d_v || !d_gate || (delta && !d_beta) ||
       (d_out && !d_q) || (!d_out && !d_state_out))
     return set_error(SI_HIP_ERR_NULL, "device state scan argument is null");
-  if (d_out && (d_out == d_q || d_out == d_k || d_out == d_v || d_out == d_gate ||
-                d_out == d_beta || d_out == d_state || d_out == d_state_out))
-    return set_error(SI_HIP_ERR_RANGE, "state scan writes what it reads");
-  if (d_state_out && (d_state_out == d_q || d_state_out == d_k || d_state_out == d_v ||
-                      d_state_out == d_gate || d_state_out == d_beta))
+  const size_t rows = sequences * tokens, gates = 4 * (size_t)scan->value_heads;
+  const size_t held = 4 * value_row * scan->key_dim;
+  const Region out(d_out, rows, 4 * value_row, 4 * value_row);
+  const Region state(d_state, sequences, held, held), state_out(d_state_out, sequences, held, held);
+  const Region in[] = {Region(d_out ? d_q : nullptr, rows, 4 * q_token_stride, 4 * key_row),
+                       Region(d_k, rows, 4 * k_token_stride, 4 * key_row),
+                       Region(d_v, rows, 4 * v_token_stride, 4 * value_row),
+                       Region(d_gate, rows, gates, gates),
+                       Region(delta ? d_beta : nullptr, rows, gates, gates),
+                       Region(scan->d_decay, gates), Region(scan->d_bias, gates),
+                       Region(scan->d_skip, gates), Region(d_counts, 4 * sequences)};
+  if (overlaps_any(out, in) || overlaps_any(state_out, in) || overlap(out, state) ||
+      overlap(out, state_out) || (d_state_out != d_state && overlap(state_out, state)))
     return set_error(SI_HIP_ERR_RANGE, "state scan writes what it reads");
   const ScanArgs a{delta,
                    scan->head_order == SI_HIP_SCAN_TILED,

@@ -488,3 +488,24 @@ def test_short_rows(hip_ctx, dev, tokens, dk, which, size, eps):
     got, new = run(hip_ctx, dev, scan)
     check_out(got, out, out_tol)
     within(new, state, state_tol, "state")
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_outputs_behind_the_inputs(hip_ctx, dev, tokens):
+    """A buffer that ends where the next begins; without outputs, queries that are the state."""
+    scan = M.Scan(np.random.default_rng(47), 1, tokens, 2, 4, 64, 32)
+    out, out_tol, state, state_tol = scan.run()
+    scan.put(dev)
+    rows = np.concatenate([x.reshape(tokens, -1) for x in (scan.q, scan.k, scan.v)], 1)
+    space = np.zeros(rows.size + out.size + scan.state.size, np.float32)
+    space[:rows.size], space[rows.size + out.size:] = rows.reshape(-1), scan.state.reshape(-1)
+    d = dev.put(space)
+    at = dict(d_q=d, d_k=d + 4 * 128, d_v=d + 8 * 128)
+    d_out, d_state = d + 4 * rows.size, d + 4 * (rows.size + out.size)
+    scan.call(hip_ctx, d_state, None, d_out, **at)
+    scan.call(hip_ctx, d_state, d_state, None, **{**at, "d_q": d_state})
+    hip_ctx.synchronize()
+    got = dev.get(d, space)
+    assert np.array_equal(got[:rows.size], space[:rows.size])
+    check_out(got[rows.size:rows.size + out.size].reshape(out.shape), out, out_tol)
+    within(got[rows.size + out.size:].reshape(state.shape), state, state_tol, "state")

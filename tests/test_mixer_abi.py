@@ -186,3 +186,37 @@ def test_conv_in_one_buffer():
         assert shared(conv_at(x=at, y=y, ys=90))
     assert shared(conv_at(x=at, y=at + 4 * 50, ys=100)) and shared(conv_at(x=at, y=at + 4 * 45, ys=91))
     assert shared(conv_at(x=at, out=at + 4 * 40, channels=40))
+
+
+SCAN = dict(sequences=3, tokens=5, qs=150, ks=160, vs=210, rule=0)
+SCAN_SIZES = dict(q=4 * (14 * 150 + 128), k=4 * (14 * 160 + 128), v=4 * (14 * 210 + 192), gate=4 * 60, beta=4 * 60,
+                  state=4 * 3 * 4 * 64 * 48, decay=16, bias=16, skip=16, n=12, state_out=4 * 3 * 4 * 64 * 48,
+                  out=4 * 15 * 192)
+
+
+def scan_at(**more):
+    a = {**{k: ROOM * (i + 1) for i, k in enumerate(SCAN_SIZES)}, **SCAN, **more}
+    h = shape(d_decay=a["decay"], d_bias=a["bias"], d_skip=a["skip"], rule=a["rule"])
+    return si_hip.lib().si_hip_state_scan_device(
+        CONTEXT, h, a["sequences"], a["tokens"], a["n"], 0, a["q"], a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["gate"],
+        a["beta"], a["state"], a["state_out"], a["out"])
+
+
+@pytest.mark.parametrize("read", ["q", "k", "v", "gate", "beta", "decay", "bias", "skip", "n", "state"])
+@pytest.mark.parametrize("written", ["out", "state_out"])
+def test_scan_outputs_apart(read, written):
+    """At the first byte that is shared and the last, from either side."""
+    at = 64 * ROOM
+    for where in (at, at + 4, at + SCAN_SIZES[read] - 4, at - SCAN_SIZES[written] + 4):
+        if (read, written, where) != ("state", "state_out", at):
+            assert shared(scan_at(**{read: at, written: where})), where
+    assert shared(scan_at(out=at, state_out=at + SCAN_SIZES["out"] - 4))
+
+
+def test_scan_in_one_buffer():
+    """Queries, keys and values in the rows of one buffer, and an output that begins among them."""
+    at = 64 * ROOM
+    qkv = dict(q=at, k=at + 4 * 128, v=at + 8 * 128, qs=448, ks=448, vs=448)
+    for more in (dict(out=at + 8 * 128 + 4), dict(out=at + 4 * 448), dict(state_out=at + 4 * 447)):
+        assert shared(scan_at(**qkv, **more))
+    assert shared(scan_at(rule=1, beta=None, gate=at, out=at + 236))
