@@ -160,7 +160,8 @@ int si_hip_rope_axis_table(size_t rotary_dim, const uint32_t *sections, size_t a
 
 /* si_hip_rope_device with the heads' norm before the rotation, and positions of one
  * or several axes: d_positions[axis * tokens + t].  norm NULL: rotation alone; rope NULL: the norm
- * alone (no axes, no positions).  One of the two is there.  d_y may be d_x with the same strides. */
+ * alone (no axes, no positions).  One of the two is there.  d_y may be d_x with the same strides;
+ * other rows of it that share memory with d_x, or with a parameter, are refused. */
 int si_hip_norm_rope_device(si_hip_context *ctx, const si_hip_head_norm *norm,
                             const si_hip_rope *rope, const si_hip_rope_axes *axes,
                             const float *d_x, size_t tokens, size_t heads, size_t head_dim,
@@ -170,7 +171,8 @@ int si_hip_norm_rope_device(si_hip_context *ctx, const si_hip_head_norm *norm,
 /* si_hip_rope_append_device with the norms of query and key heads before their rotation, in
  * the same launch, and positions of one or several axes: d_positions[axis * sequences * tokens +
  * s * tokens + t] (NULL: the slots' numbers, on every axis).  norm NULL: none.  Query rows need a
- * norm or a rotation. */
+ * norm or a rotation.  d_q_out that shares memory with k, v, a parameter or, but for d_q itself, q is
+ * refused. */
 int si_hip_norm_rope_append_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
                                    const si_hip_head_norm *norm, const si_hip_rope *rope,
                                    const si_hip_rope_axes *axes, size_t tokens,

@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "decode_internal.h"
+#include "overlap.h"
 #include "si_hip_status.h"
 
 using namespace sihip;
@@ -94,6 +95,19 @@ int check_norm_rope(const si_hip_head_norm *norm, const si_hip_rope *rope,
     *a = AxesArgs{axes->axes, axes->d_axis};
   }
   return SI_HIP_OK;
+}
+
+// A stride of floats in bytes (one that passes the address space is at its end: only a single row has it).
+size_t in_bytes(size_t floats) { return floats > SIZE_MAX / 4 ? SIZE_MAX : 4 * floats; }
+
+// Whether rows that a normed rotation writes share memory with its parameters.
+bool overlaps_norm_rope(const Region &out, const NormArgs &n, const RopeArgs &r, const AxesArgs &a,
+                        size_t head_dim, const uint32_t *d_positions, size_t rows) {
+  const Region in[] = {Region(n.q, 4 * head_dim), Region(n.k, 4 * head_dim),
+                       Region(r.frequencies, 4 * (size_t)r.rotary_dim),
+                       Region(a.axis, r.rotary_dim / 2u),
+                       Region(r.rotary_dim ? d_positions : nullptr, 4 * a.axes * rows)};
+  return overlaps_any(out, in);
 }
 
 // sequences * tokens rows of a step: within the kernels' 31 bits
@@ -296,6 +310,14 @@ int si_hip_norm_rope_device(si_hip_context *ctx, const si_hip_head_norm *norm,
     return set_error(SI_HIP_ERR_NULL, "device head norm argument is null");
   if (d_x == d_y && (token_stride != y_token_stride || head_stride != y_head_stride))
     return set_error(SI_HIP_ERR_DIMENSIONS, "head norm in place needs one set of strides");
+  const Region x(d_x, tokens, in_bytes(token_stride), heads, in_bytes(head_stride), 4 * head_dim);
+  const Region y(d_y, tokens, in_bytes(y_token_stride), heads, in_bytes(y_head_stride),
+                 4 * head_dim);
+  // (the keys' weight is not read)
+  n.k = nullptr;
+  if ((d_x != d_y && overlap(y, x)) ||
+      overlaps_norm_rope(y, n, r, a, head_dim, d_positions, tokens))
+    return set_error(SI_HIP_ERR_RANGE, "head norm writes what it reads");
   const RopeRows rows{d_x, d_y, token_stride, head_stride, y_token_stride, y_head_stride,
                       (uint32_t)heads};
   return submit(ctx, "head norm launch", [&](const Workspace &ws, hipStream_t s, bool) {
@@ -333,6 +355,19 @@ int si_hip_norm_rope_append_device(si_hip_context *ctx, const si_hip_kv_cache *c
   }
   if (!ctx || !d_k || !d_v) return set_error(SI_HIP_ERR_NULL, "cache append argument is null");
   if ((rc = check_cache_buffers(view)) != 0) return rc;
+  if (d_q) {
+    const size_t rows = view.sequences * tokens, row = 4 * view.kv_heads * dim;
+    const Region out(d_q_out, 4 * rows * heads * dim);
+    const Region in[] = {Region(d_k, rows, in_bytes(k_token_stride), row),
+                         Region(d_v, rows, in_bytes(v_token_stride), row),
+                         Region(d_q_out != d_q ? d_q : nullptr, rows, in_bytes(q_token_stride),
+                                heads, in_bytes(q_head_stride), 4 * dim),
+                         Region(d_counts, 4 * (size_t)view.sequences),
+                         Region(view.table, 4 * (size_t)view.sequences * view.max_pages),
+                         Region(view.lengths, 4 * (size_t)view.sequences)};
+    if (overlaps_any(out, in) || overlaps_norm_rope(out, n, r, a, dim, d_positions, rows))
+      return set_error(SI_HIP_ERR_RANGE, "cache append writes what it reads");
+  }
   const RopeRows q{d_q, d_q_out, q_token_stride, q_head_stride, heads * dim, dim, (uint32_t)heads};
   return submit(ctx, "cache append launch", [&](const Workspace &ws, hipStream_t s, bool) {
     return launch_norm_rope_append(view, n, r, a, (uint32_t)tokens, d_counts, d_positions, d_k,

@@ -250,3 +250,25 @@ def test_reports(hip_ctx, dev):
             assert np.allclose(R.decode(keys[p, :, o], "f16")[:, rows], wk[4 + t][:, rows], rtol=2e-3,
                                atol=2e-3)
     hip_ctx.synchronize()
+
+
+def test_rows_beside_one_another(hip_ctx, dev):
+    """Heads beside the gates of their outputs, normed into the gates' places and into a buffer that ends
+    where theirs begins."""
+    rng = np.random.default_rng(8)
+    tokens, heads, dim = 9, 5, 64
+    c = Call(dev, rng, tokens, dim, 32, 0, [6, 10], 0, "plain")
+    x = rng.standard_normal((tokens, heads, 2, dim)).astype(np.float32)
+    want, size = c.want(x[:, :, 0], 0)
+    space = np.concatenate([np.zeros(tokens * heads * dim, np.float32), x.reshape(-1)])
+    d = dev.put(space)
+    d_x = d + 4 * tokens * heads * dim
+    args = dict(norm=c.norm, rope=c.rope, axes=c.axes, d_positions=c.d_positions, head_stride=2 * dim)
+    hip_ctx.norm_rope_device(d_x, tokens, heads, dim, d, **args)
+    hip_ctx.norm_rope_device(d_x, tokens, heads, dim, d_x + 4 * dim, y_head_stride=2 * dim, **args)
+    hip_ctx.synchronize()
+    got = dev.get(d, space)
+    check(got[:tokens * heads * dim].reshape(want.shape), want, size)
+    got = got[tokens * heads * dim:].reshape(x.shape)
+    check(got[:, :, 1], want, size)
+    assert np.array_equal(got[:, :, 0], x[:, :, 0])

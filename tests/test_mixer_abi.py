@@ -220,3 +220,49 @@ def test_scan_in_one_buffer():
     for more in (dict(out=at + 8 * 128 + 4), dict(out=at + 4 * 448), dict(state_out=at + 4 * 447)):
         assert shared(scan_at(**qkv, **more))
     assert shared(scan_at(rule=1, beta=None, gate=at, out=at + 236))
+
+
+ROWS_SIZES = dict(x=4 * (2 * 700 + 7 * 80 + 64), qw=256, freq=256, axis=32, pos=4 * 9)
+
+
+def rows_at(**more):
+    a = {**{k: ROOM * (i + 1) for i, k in enumerate([*ROWS_SIZES, "kw", "y"])},
+         **dict(ts=700, hs=80, yts=900, yhs=96, one=False), **more}
+    return si_hip.lib().si_hip_norm_rope_device(
+        CONTEXT, norm(d_q_weight=a["qw"], d_k_weight=a["kw"]), rope(d_frequencies=a["freq"]),
+        None if a["one"] else axes(d_axis=a["axis"]), a["x"], 3, 8, 64, a["ts"], a["hs"], a["pos"], a["y"], a["yts"],
+        a["yhs"])
+
+
+@pytest.mark.parametrize("read", ROWS_SIZES)
+def test_rows_outputs_apart(read):
+    at, size = 64 * ROOM, 4 * (2 * 900 + 7 * 96 + 64)
+    for where in (at, at + 4, at + ROWS_SIZES[read] - 4, at - size + 4):
+        if (read, where) != ("x", at):
+            assert shared(rows_at(**{read: at, "y": where})), where
+    assert shared(rows_at(x=at, y=at + 4, yts=700, yhs=80)) and shared(rows_at(x=at, y=at + 4 * 79, yts=700, yhs=80))
+    assert shared(rows_at(pos=at, y=at - size + 4, one=True)) and rows_at(x=at, y=at) == DIM
+
+
+APPEND_SIZES = dict(k=4 * (5 * 300 + 256), v=4 * (5 * 310 + 256), q=4 * (5 * 1300 + 7 * 128 + 64), pos=72, qw=256,
+                    kw=256, freq=256, axis=32, n=8, table=32, lengths=8)
+
+
+def append_at(**more):
+    a = {**{k: ROOM * (i + 1) for i, k in enumerate([*APPEND_SIZES, "qo"])}, **dict(ks=300, vs=310, qs=1300, qh=128),
+         **more}
+    return si_hip.lib().si_hip_norm_rope_append_device(
+        CONTEXT, cache(d_page_table=a["table"], d_lengths=a["lengths"]), norm(d_q_weight=a["qw"], d_k_weight=a["kw"]),
+        rope(d_frequencies=a["freq"]), axes(d_axis=a["axis"]), 3, a["n"], a["pos"], a["k"], a["ks"], a["v"], a["vs"],
+        a["q"], 8, a["qs"], a["qh"], a["qo"])
+
+
+@pytest.mark.parametrize("read", APPEND_SIZES)
+def test_append_outputs_apart(read):
+    at, size = 64 * ROOM, 4 * 6 * 512
+    for where in (at, at + 4, at + APPEND_SIZES[read] - 4, at - size + 4):
+        if (read, where) != ("q", at):
+            assert shared(append_at(**{read: at, "qo": where})), where
+    assert append_at(q=at, qo=at) == DIM
+    # q, k and v in one row, the outputs among them
+    assert shared(append_at(q=at, qs=1024, qh=64, k=at + 2048, ks=1024, v=at + 3072, vs=1024, qo=at + 4096 * 5 + 2048))
