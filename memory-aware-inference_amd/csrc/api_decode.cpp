@@ -89,7 +89,7 @@ int check_norm_rope(const si_hip_head_norm *norm, const si_hip_rope *rope,
   }
   if (axes) {
     if (!rope) return set_error(SI_HIP_ERR_NULL, "rotary axes need a rotary description");
-    if (axes->axes == 0 || axes->axes > SI_HIP_MAX_ROPE_AXES)
+    if (axes->axes == 0 || axes->axes > SI_HIP_MAX_ROPE_AXES || axes->reserved != 0)
       return set_error(SI_HIP_ERR_DIMENSIONS, "rotary axes are invalid");
     if (!axes->d_axis) return set_error(SI_HIP_ERR_NULL, "rotary axis table is null");
     *a = AxesArgs{axes->axes, axes->d_axis};

@@ -109,8 +109,8 @@ struct NormArgs {
   bool on;                     // false: no norm
 };
 struct AxesArgs {
-  uint32_t axes;               // 1: no table is read
-  const uint8_t* axis;
+  uint32_t axes;
+  const uint8_t* axis;         // of each pair; null: all on axis 0
 };
 hipError_t launch_norm_rope(const NormArgs& norm, const RopeArgs& rope, const AxesArgs& axes,
                             const RopeRows& rows, uint32_t tokens, uint32_t head_dim,

@@ -272,3 +272,24 @@ def test_rows_beside_one_another(hip_ctx, dev):
     got = got[tokens * heads * dim:].reshape(x.shape)
     check(got[:, :, 1], want, size)
     assert np.array_equal(got[:, :, 0], x[:, :, 0])
+
+
+def test_one_axis_has_a_table(hip_ctx, dev):
+    """A table for one axis is read like any other: zeros are axis 0, an entry beyond it is reported."""
+    rng = np.random.default_rng(9)
+    c = Call(dev, rng, 3, 64, 32, 0, [16], 0, "plain")
+    x = rng.standard_normal((3, 2, 64)).astype(np.float32)
+    want, size = c.want(x, 0)
+    args = dict(norm=c.norm, rope=c.rope, d_positions=c.d_positions)
+    d_x, d_y = dev.put(x), dev.put(x)
+    hip_ctx.norm_rope_device(d_x, 3, 2, 64, d_y, axes=c.axes, **args)
+    hip_ctx.synchronize()
+    check(dev.get(d_y, x), want, size)
+    table = c.axis.copy()
+    table[3] = 1
+    bad = si_hip.RopeAxes(axes=1, d_axis=dev.put(table))
+    hip_ctx.norm_rope_device(d_x, 3, 2, 64, d_y, axes=bad, **args)
+    with pytest.raises(HipError) as e:
+        hip_ctx.synchronize()
+    assert e.value.status == -9
+    check(dev.get(d_y, x), want, size)

@@ -266,3 +266,9 @@ def test_append_outputs_apart(read):
     assert append_at(q=at, qo=at) == DIM
     # q, k and v in one row, the outputs among them
     assert shared(append_at(q=at, qs=1024, qh=64, k=at + 2048, ks=1024, v=at + 3072, vs=1024, qo=at + 4096 * 5 + 2048))
+
+
+@pytest.mark.parametrize("call", [rows, append])
+def test_reserved_of_axes(call):
+    assert call(a=axes(reserved=1)) == DIM and "rotary axes" in si_hip.last_error()
+    assert call(a=axes(axes=1)) == NULL and "argument is null" in si_hip.last_error()
