@@ -1122,15 +1122,22 @@ Shape shape_for(const ScanArgs& a) {
 
 }  // namespace
 
-// (A chunk's rows lie within the 2^30 bytes that its buffers' offsets reach.)  Eight tokens, or four
-// where one round of workgroups takes them, are faster than token by token: 48 heads of 128, chunks / steps,
-// 4 tokens of one sequence 9.3 / 11.4 us, of four 12.3 / 13.5, of 16 37.0 / 31.5; 8 tokens
-// 9.3 / 16.4, 12.4 / 19.0, 38.2 / 43.5; 3 tokens of four 12.3 / 12.2.
+// (A chunk's rows lie within the 2^30 bytes that its buffers' offsets reach.)  Where one round of workgroups takes
+// them four tokens are faster in a chunk than token by token: 48 heads of 128 x 128, delta rule, chunks /
+// steps, 4 tokens of one sequence 7.6 / 11.2 us, of four 10.8 / 13.0; of 64 x 64 6.1 / 7.5, 6.7 / 8.0; of one sequence of 256 x 128
+// 10.4 / 14.4.  With more rounds a chunk costs the same for all lengths, steps by the state: 48 sequences of 48
+// heads, 8, 12 and 16 tokens, 128 x 128 96 / 95, 96 / 124, 97 / 150; 64 x 128 64 / 44, 63 / 57, 63 / 69;
+// 96 x 96 76 / 59, 76 / 79, 76 / 96; 64 x 64 50 / 29, 50 / 38, 51 / 46; 32 x 128 50 / 29, 50 / 40, 50 / 48. 12
+// sequences: 128 x 128 32 / 38, 33 / 49, 33 / 59; 64 x 128 21 / 19, 22 / 25, 22 / 30; 64 x 64 17 / 14, 18 / 19, 18 / 23.
+// The selective form the same way: 48 sequences 128 x 128 79 / 84, 79 / 105, 80 / 124; 64 x 128 50 / 39, 50 / 48,
+// 49 / 56; 64 x 64 41 / 25, 41 / 32, 42 / 38.
 bool scan_chunks_take(const ScanArgs& a) {
   constexpr size_t most = size_t(1) << 23;
+  const uint32_t state = a.key_dim * a.value_dim;
+  const uint32_t enough = state >= 128u * 128u ? 8u : state > 64u * 64u ? 12u : 16u;
   return a.k_stride <= most && a.v_stride <= most &&
          (!a.out || (a.q_stride <= most && (size_t)a.value_heads * a.value_dim <= most)) &&
-         (a.count.tokens >= 8u || (a.count.tokens >= 4u && shape_for(a).rounds == 1u));
+         (a.count.tokens >= enough || (a.count.tokens >= 4u && shape_for(a).rounds == 1u));
 }
 
 hipError_t launch_scan_chunks(const ScanArgs& a, hipStream_t s) {

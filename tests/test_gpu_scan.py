@@ -509,3 +509,16 @@ def test_outputs_behind_the_inputs(hip_ctx, dev, tokens):
     assert np.array_equal(got[:rows.size], space[:rows.size])
     check_out(got[rows.size:rows.size + out.size].reshape(out.shape), out, out_tol)
     within(got[rows.size + out.size:].reshape(state.shape), state, state_tol, "state")
+
+
+@pytest.mark.parametrize("rule", [DELTA, SELECTIVE])
+@pytest.mark.parametrize("dk,dv", [(32, 64), (64, 64), (64, 72), (64, 128), (128, 120), (128, 128)])
+def test_short_calls_of_many_heads(hip_ctx, dev, dk, dv, rule):
+    """Around the lengths from which calls of several rounds are taken in chunks."""
+    for tokens in (7, 8, 11, 12, 15, 16):
+        scan = M.Scan(np.random.default_rng(tokens), 6, tokens, 2, 90, dk, dv, rule,
+                      counts=[tokens, 0, tokens - 1, 1, tokens, tokens])
+        out, out_tol, state, state_tol = scan.run()
+        got, new = run(hip_ctx, dev, scan)
+        check_out(got, out, out_tol)
+        within(new, state, state_tol, "state")
