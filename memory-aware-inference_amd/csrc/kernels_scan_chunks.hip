@@ -59,13 +59,13 @@ constexpr float kForgotten = -256.0f; // the least log decay of a token
 // The waves of a workgroup: `takers` that take sixteen columns each through the chunks, two or four that
 // make the rows of K and Q, and two that make what is left of a chunk's operands.  Four makers of
 // rows where two takers leave registers for eight waves: theirs is the longest course without the
-// correction (3001 tokens of 64 heads of 128 x 64: 205 us with two, 190 with four), and close
-// to it else (4093 tokens of 48 heads of 128: 310 and 294).
-constexpr uint32_t row_makers(uint32_t steps, bool delta, uint32_t takers) {
+// correction (two sequences of 3001 tokens of 64 heads of 128 x 64: 208 us with two, 186 with four), and close
+// to it with it (4093 tokens of 48 heads of 128: 303 and 293).
+constexpr uint32_t row_makers(uint32_t steps, uint32_t takers) {
   return steps > 2 && takers == 2 ? 4 : 2;
 }
-constexpr uint32_t waves_of(uint32_t steps, bool delta, uint32_t takers) {
-  return takers + 2u + row_makers(steps, delta, takers);
+constexpr uint32_t waves_of(uint32_t steps, uint32_t takers) {
+  return takers + 2u + row_makers(steps, takers);
 }
 constexpr uint32_t kRow = 20;     // floats between rows of the 16 x 16 blocks of f32
 
@@ -918,8 +918,8 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
 // At step n of its course chunk n's rows and gates and chunk n - 1's blocks are made, and chunk n - 2 is taken;
 // where LDS is tight, chunk n's rows and gates while chunk n - 1 is taken, then chunk n's blocks.
 template <uint32_t STEPS, bool DELTA, uint32_t TAKERS>
-__global__ __launch_bounds__(64 * waves_of(STEPS, DELTA, TAKERS))
-__attribute__((amdgpu_waves_per_eu(waves_of(STEPS, DELTA, TAKERS) / 4))) void scan_chunks_kernel(ScanArgs a,
+__global__ __launch_bounds__(64 * waves_of(STEPS, TAKERS))
+__attribute__((amdgpu_waves_per_eu(waves_of(STEPS, TAKERS) / 4))) void scan_chunks_kernel(ScanArgs a,
                                                                               uint32_t blocks) {
   __shared__ ChunkShared<STEPS> sh;
   constexpr bool TIGHT = ChunkShared<STEPS>::kTight;
@@ -934,7 +934,7 @@ __attribute__((amdgpu_waves_per_eu(waves_of(STEPS, DELTA, TAKERS) / 4))) void sc
   const uint32_t dk = a.key_dim, dv = a.value_dim;
   if (wave >= TAKERS + 2u) {
     const uint32_t maker = wave - TAKERS - 2u, key_head = key_head_of(a, head);
-    constexpr uint32_t MAKERS = row_makers(STEPS, DELTA, TAKERS);
+    constexpr uint32_t MAKERS = row_makers(STEPS, TAKERS);
     using W = Raw<STEPS, MAKERS>;
     W raw;
     const float* k = a.k + row0 * a.k_stride + (size_t)key_head * dk;
@@ -1077,10 +1077,10 @@ hipError_t launch(const ScanArgs& a, hipStream_t s) {
       return hipErrorInvalidValue;
     else if (a.delta)
       scan_chunks_kernel<STEPS, true, TAKERS>
-          <<<grid, 64u * waves_of(STEPS, true, TAKERS), 0, s>>>(a, blocks);
+          <<<grid, 64u * waves_of(STEPS, TAKERS), 0, s>>>(a, blocks);
     else
       scan_chunks_kernel<STEPS, false, TAKERS>
-          <<<grid, 64u * waves_of(STEPS, false, TAKERS), 0, s>>>(a, blocks);
+          <<<grid, 64u * waves_of(STEPS, TAKERS), 0, s>>>(a, blocks);
     return hipGetLastError();
   };
   using std::integral_constant;
@@ -1096,9 +1096,11 @@ hipError_t launch(const ScanArgs& a, hipStream_t s) {
 
 // Columns a workgroup has: the more, the fewer make the same operands twice, but the longer a chunk takes
 // (two, four and eight takers 5, 6 and 9 thousand cycles, key_dim 128) and the fewer workgroups there
-// are for the card's 256 CUs, each of which holds one: what takes the fewest cycles in whole rounds.
-// One prompt of 2048 tokens, 48 heads of 128: 165 us with two, 182 with four, 248 with eight; two of them
-// 325, 200, 268; four of 1024 263, 206, 163; sixteen of 512 542, 374, 285.
+// are for the card's 256 CUs, each of which holds one: what takes the fewest cycles in whole rounds.  (Below 33 keys LDS
+// has room for two, but 192 workgroups take 61 us and 384 of them 113.)  1024 tokens of 48 heads of 128 x 128, delta rule: one sequence 83 us with two, 90 with four, 125 with
+// eight; two of them 153, 92, 125; four 230, 180, 131; eight 458, 302, 268.  The same order within 4 % for keys of
+// 32, 64 and 256 and the selective form: four sequences of 32 keys 166, 136, 90, of 64 184, 157, 104, of 256 502,
+// 373 (no eight); selective ones 117, 63, 59, 136, 99, 68, 337, 307, of 128 184, 142, 100.
 struct Shape {
   uint32_t takers;
   uint64_t rounds;
