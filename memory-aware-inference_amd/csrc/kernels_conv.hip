@@ -14,8 +14,13 @@ namespace {
 constexpr uint32_t kThreads = 64;
 constexpr uint32_t kStep = 8;  // tokens whose inputs are under way together
 
+// y / (1 + e^-y).  The quotient by the card's reciprocal, good to a unit in the last place, and what it leaves of y taken
+// into it: to half a unit, as a division's.  500 tokens of 10240 channels take 10.3 us (without it 9.75, by a division
+// 11.3), 2000 29.4 (28.9, 29.3).
 __device__ __forceinline__ float silu(float y) {
-  return y * __builtin_amdgcn_rcpf(1.0f + expf(-y));  // (the card's reciprocal: a unit in the last place)
+  const float d = 1.0f + expf(-y), r = __builtin_amdgcn_rcpf(d), q = y * r;
+  const float z = __builtin_fmaf(__builtin_fmaf(-q, d, y), r, q);
+  return d < __builtin_inff() ? z : q;
 }
 
 template <uint32_t N>

@@ -163,3 +163,21 @@ def test_rows_beside_one_another(hip_ctx, dev):
     check(got[..., 1:channels + 1], want, tol)
     got[..., 1:channels + 1] = 9.0
     assert np.array_equal(got, rows) and np.array_equal(dev.get(d_state, states), states)
+
+
+def test_activation(hip_ctx, dev):
+    """SiLU of values from 9 to 17, where e^-y is below 2^-12 and its own error below 2^-11 U of the sum: the sum and
+    the quotient round to half a step, U each, and what corrects the quotient adds less than 2^-20 U. And of any
+    finite value, with the exponential's error of up to 2 U."""
+    rng = np.random.default_rng(10)
+    channels = 1 << 16
+    w = np.zeros((channels, 2), np.float32)
+    w[:, 1] = 1.0
+    for low, high, tol in [(9.0, 17.0, 2.001 * M.U), (-80.0, 9.0, 4.001 * M.U), (-3.4e38, 3.4e38, 2.001 * M.U)]:
+        y = rng.uniform(low, high, (1, channels)).astype(np.float32)
+        d_out = dev.put(np.zeros_like(y))
+        hip_ctx.causal_conv_device(dev.put(y), dev.put(w), 1, 1, channels, 2, d_y=d_out)
+        hip_ctx.synchronize()
+        want = M.silu(y.astype(np.float64))
+        err = np.abs(dev.get(d_out, y) - want)
+        assert np.all(err <= tol * np.abs(want) + 1e-36), np.max(err / (np.abs(want) + 1e-36)) / M.U
