@@ -348,7 +348,8 @@ __device__ __forceinline__ void make_rows(ChunkShared<STEPS>& sh, uint32_t chunk
     const float sum = reduced<W::kLanes>(x, lane, [](float y, float z) { return y + z; });
     // (rows behind the last token are zeros whatever eps is)
     scale = kUp * inverse_root(sum + (token < left ? a.eps : 1.0f));
-    bool small = token < left && sum < a.eps * 0x1p-16f;
+    // (queries that are not read are zeros)
+    bool small = token < left && sum < a.eps * 0x1p-16f && (a.out || in % 2u == 0u);
     bool some = false;
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(small) != 0u, 0)) {
       const float most = sizes();
