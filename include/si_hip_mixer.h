@@ -89,8 +89,11 @@ typedef struct si_hip_state_scan {
  * States, sums and decays are f32, or wider.  Single tokens, and rows more than 2^23
  * floats apart, are taken token by token in f32; prompts and most calls of four
  * tokens and more in chunks of 32 on the matrix cores, each f32 operand as a sum of two f16 (22 bits of the
- * largest value of its row or column) or three bf16 (all of its bits).  What a chunk forgets
- * to less than 2^-126 of it within 32 tokens counts as forgotten, and none grows to 2^127 times what it was. */
+ * largest value of its row or column) or three bf16 (all of its bits), but for
+ * SI_HIP_KERNEL_GENERIC: f32 token by token.  What a chunk forgets
+ * to less than 2^-126 of it within 32 tokens counts as forgotten, and none grows to 2^127 times what it was.
+ * DELTA: a row's squares are added up in f32 (with eps the sum has to be 2^-126 at least, and finite);
+ * chunks with a row, but for zeros, that is shorter than 2^-8 of eps's root are taken token by token. */
 int si_hip_state_scan_device(si_hip_context *ctx, const si_hip_state_scan *scan, size_t sequences,
                              size_t tokens, const uint32_t *d_counts, uint32_t more,
                              const float *d_q, size_t q_token_stride, const float *d_k,

@@ -265,7 +265,8 @@ def test_append_outputs_apart(read):
             assert shared(append_at(**{read: at, "qo": where})), where
     assert append_at(q=at, qo=at) == DIM
     # q, k and v in one row, the outputs among them
-    assert shared(append_at(q=at, qs=1024, qh=64, k=at + 2048, ks=1024, v=at + 3072, vs=1024, qo=at + 4096 * 5 + 2048))
+    row = dict(q=at, qs=1100, qh=64, k=at + 2064, ks=1100, v=at + 3100, vs=1100)
+    assert shared(append_at(**row, qo=at + 4400 * 5 + 2064)) and shared(append_at(**row, qo=at + 4400 * 5 + 4120))
 
 
 @pytest.mark.parametrize("call", [rows, append])

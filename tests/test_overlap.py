@@ -47,8 +47,8 @@ int main() {
   }
   // none, the whole address space, more rows than a loop could take
   const Region none(nullptr, 8), all((void*)16, size_t(1) << 40, size_t(1) << 40, 4);
-  const Region q((void*)0x10000, size_t(1) << 31, 3072, 1024), k((void*)0x10400, size_t(1) << 31, 3072, 2048);
-  const Region over((void*)0x10400, size_t(1) << 31, 3072, 2049);
+  const Region q((void*)0x10000, size_t(1) << 31, 3200, 1024), k((void*)0x10400, size_t(1) << 31, 3200, 2176);
+  const Region over((void*)0x10400, size_t(1) << 31, 3200, 2177);
   if (sihip::overlap(none, all) || sihip::overlap(all, none) || !sihip::overlap(all, all) ||
       sihip::overlap(q, k) || !sihip::overlap(q, over) || all.end != UINTPTR_MAX)
     return 2;
