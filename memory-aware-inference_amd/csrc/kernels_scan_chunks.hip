@@ -181,6 +181,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const float* first, si
   return buffer_of(first, min(left, kChunk) * (uint32_t)stride * 4u);
 }
 
+constexpr uint32_t kRaised = 1u, kZeros = 2u;  // short rows that are raised, keys that are zeros
 struct alignas(16) Gated {  // of a chunk's tokens (four of them are read at once)
   float grow[kChunk];   // e^{G_i}
   float fade[kChunk];   // e^{G - G_i}
@@ -188,7 +189,7 @@ struct alignas(16) Gated {  // of a chunk's tokens (four of them are read at onc
   float keep[kChunk];   // a_i
   float key[kChunk], query[kChunk];  // what the rows of the operands are to be multiplied by
   float total;          // e^{G}
-  // of eight rows each: whether some are raised, and all have key[], query[] (delta rule)
+  // of eight rows each (delta rule): kRaised, kZeros, or nothing; rows beside these have key[], query[]
   alignas(4) uint8_t raised[4];
 };
 
@@ -350,16 +351,19 @@ __device__ __forceinline__ void make_rows(ChunkShared<STEPS>& sh, uint32_t chunk
     scale = kUp * inverse_root(sum + (token < left ? a.eps : 1.0f));
     // (queries that are not read are zeros)
     bool small = token < left && sum < a.eps * 0x1p-16f && (a.out || in % 2u == 0u);
-    bool some = false;
+    uint32_t some = 0u;
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(small) != 0u, 0)) {
       const float most = sizes();
-      small = small && most > 0.0f;  // (zeros are held as they are)
-      some = __builtin_amdgcn_ballot_w64(small) != 0u;
+      const bool none = small && !(most > 0.0f);  // (zeros are held as they are)
+      small = small && !none;
+      some = (__builtin_amdgcn_ballot_w64(small) ? kRaised : 0u) |
+             (__builtin_amdgcn_ballot_w64(none && in % 2u == 0u) ? kZeros : 0u);
       // (the largest into [2^8, 2^10); what is below 2^-118 has fewer bits)
       const int32_t e = exponent(scale);
       const int32_t up = small ? max(min(min(262 - exponent(most) - e, 253 - e), 126), 0) : 0;
       scale *= __uint_as_float((uint32_t)(127 + up) << 23);
-      if (in < V) (in % 2u ? g.query : g.key)[token] = __uint_as_float((uint32_t)(127 - up) << 23);
+      const float down = none ? 0.0f : __uint_as_float((uint32_t)(127 - up) << 23);
+      if (in < V) (in % 2u ? g.query : g.key)[token] = down;
     }
 #pragma unroll
     for (uint32_t i = 0; i < W::kPartRows / 8u; ++i) g.raised[part * (W::kPartRows / 8u) + i] = some;
@@ -797,7 +801,9 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
     put(u[0], 0u);
     put(u[1], 1u);
   }
-  bool odd = DELTA && *reinterpret_cast<const uint32_t*>(g.raised);
+  const uint32_t raised =
+      DELTA ? __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t*>(g.raised)) : 0u;
+  bool odd = raised & (0x01010101u * kRaised);
 #pragma unroll
   for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
@@ -866,6 +872,13 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
     __builtin_amdgcn_sched_barrier(0);
   }
   float gained = 0.0f;
+  if (__builtin_expect(raised != 0u, false)) {
+    // (a key of zeros adds nothing, however large its u: the units are the others')
+#pragma unroll
+    for (uint32_t t = 0; t < 2; ++t)
+      if (raised >> (8u * (2u * t + p / 2u)) & kZeros)
+        u[t] *= *reinterpret_cast<const f32x4*>(g.key + 16u * t + 4u * p);
+  }
 #pragma unroll
   for (uint32_t t = 0; t < 2; ++t) {
     u[t] *= fade[t];

@@ -522,3 +522,20 @@ def test_short_calls_of_many_heads(hip_ctx, dev, dk, dv, rule):
         got, new = run(hip_ctx, dev, scan)
         check_out(got, out, out_tol)
         within(new, state, state_tol, "state")
+
+
+@pytest.mark.parametrize("loud", [1.0, 1e5, 1e12, 1e25])
+@pytest.mark.parametrize("tokens,dk,heads,sequences", [(3, 64, 4, 2), (12, 64, 4, 2), (70, 128, 4, 2), (70, 160, 4, 2),
+                                                       (40, 128, 70, 6)])
+def test_zero_keys(hip_ctx, dev, tokens, dk, heads, sequences, loud):
+    """Tokens whose keys are zeros leave the state what it is, whatever their values are."""
+    scan = M.Scan(np.random.default_rng(53), sequences, tokens, 2, heads, dk, 72)
+    scan.gate -= 3.0
+    scan.k[:, 1::3, 0] = 0.0
+    scan.v[:, 1::3, :heads // 2] *= np.float32(loud)  # of the heads that share these keys
+    scan.k[0, :, 1] = 0.0
+    scan.v[0, :, heads // 2:] *= np.float32(loud)
+    out, out_tol, state, state_tol = scan.run()
+    got, new = run(hip_ctx, dev, scan)
+    check_out(got, out, out_tol)
+    within(new, state, state_tol, "state")
