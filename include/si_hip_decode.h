@@ -129,7 +129,8 @@ int si_hip_kv_advance_device(si_hip_context *ctx, const si_hip_kv_cache *cache,
 
 /* ---- norms of heads, positions of several axes ------------------------------ */
 /* RMS norm of a head's values before they turn: y = x * inv * w, or with plus_one
- * x * inv * (1 + w), inv = 1 / sqrt(mean(x^2) + eps) over head_dim values; a
+ * x * inv * (1 + w), inv = 1 / sqrt(mean(x^2) + eps) over head_dim values (the
+ * squares' sum has to be within f32's range); a
  * weight that is NULL is all ones (plus_one does not apply to it). */
 typedef struct si_hip_head_norm {
   float eps;         /* finite, above 0 */

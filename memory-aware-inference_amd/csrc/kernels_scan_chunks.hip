@@ -819,11 +819,8 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
     f32x4 o[2];
 #pragma unroll
     for (uint32_t t = 0; t < 2; ++t) {
-      o[t] = grow[t] * (sq[t] * down_q) + skip * v[t];
-      if (!DELTA)
-        o[t] = grow[t] * (sq[t] * down_q) *
-                   *reinterpret_cast<const f32x4*>(g.query + 16u * t + 4u * p) +
-               skip * v[t];
+      o[t] = grow[t] * (sq[t] * down_q);
+      if (!DELTA) o[t] *= *reinterpret_cast<const f32x4*>(g.query + 16u * t + 4u * p);
     }
 #pragma unroll
     for (uint32_t i = 0; i < kPairs; ++i)
@@ -837,8 +834,9 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
       for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i)
+          // (skip v last: the sums before it are cut to their own size)
           __builtin_amdgcn_raw_buffer_store_b32(
-              __float_as_uint(o[t][i]), to,
+              __float_as_uint(__builtin_fmaf(skip, v[t][i], o[t][i])), to,
               at + (16u * t + i) * 4u * (uint32_t)c.out_stride, 0, 0);
     }
   }
