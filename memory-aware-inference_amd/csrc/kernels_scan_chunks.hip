@@ -826,6 +826,12 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
     for (uint32_t i = 0; i < kPairs; ++i)
 #pragma unroll
       for (uint32_t t = 0; t < 2; ++t) o[t] = mfma(mix[t][kLeft[i]], right[kRight[i]], o[t]);
+    // (last: the sums before it are cut to their own size)
+    if (__builtin_amdgcn_readfirstlane(__float_as_uint(skip)))
+#pragma unroll
+      for (uint32_t t = 0; t < 2; ++t)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) o[t][i] = __builtin_fmaf(skip, v[t][i], o[t][i]);
     if (c.out) {
       const __amdgpu_buffer_rsrc_t to = rows_of(c.out + t0 * c.out_stride, c.out_stride, left);
       uint32_t at = c.out_at;
@@ -834,9 +840,8 @@ __device__ __forceinline__ void take_chunk(State<STEPS>& st, const ChunkShared<S
       for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i)
-          // (skip v last: the sums before it are cut to their own size)
           __builtin_amdgcn_raw_buffer_store_b32(
-              __float_as_uint(__builtin_fmaf(skip, v[t][i], o[t][i])), to,
+              __float_as_uint(o[t][i]), to,
               at + (16u * t + i) * 4u * (uint32_t)c.out_stride, 0, 0);
     }
   }
