@@ -26,7 +26,7 @@
 //
 // A chunk of one workgroup by itself is a chain: products with the state, the system's three products,
 // P's, the units, the state's own; a taker's wave, alone on its SIMD, issues or waits for one of
-// them at a time (4093 tokens of 48 heads of 128: 128 chunks in 294 us, 5 thousand cycles each; its
+// them at a time (4093 tokens of 48 heads of 128: 128 chunks in 295 us, 5 thousand cycles each; its
 // matrix instructions are 1.6 thousand of them).  With eight takers a SIMD has three waves and a chunk 1.6 thousand
 // vector instructions of four cycles and more and 230 matrix instructions of 16: 9 thousand cycles.
 //
